@@ -1,0 +1,90 @@
+// Device helpers of the paged cache's kernels.
+
+#pragma once
+
+#include "paged.h"
+
+namespace paged {
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+struct BF16 {
+  typedef __bf16 T;
+};
+struct FP16 {
+  typedef _Float16 T;
+};
+struct E4M3 {
+  typedef uint8_t T;
+};
+
+template <class C> struct Vec {
+  typedef typename C::T x2 __attribute__((ext_vector_type(2)));
+  typedef typename C::T x4 __attribute__((ext_vector_type(4)));
+  typedef typename C::T x8 __attribute__((ext_vector_type(8)));
+};
+
+constexpr float kMinusInf = -__builtin_inff();
+
+template <class C> __device__ inline float to_float(typename C::T x) { return (float)x; }
+template <> __device__ inline float to_float<E4M3>(uint8_t x) {
+  return __builtin_amdgcn_cvt_f32_fp8(x, 0);
+}
+
+// 8 neighbours of 16 bytes (8 bytes of e4m3) in 32 bits.
+template <class C> __device__ inline void load8(const typename C::T* p, float (&x)[8]) {
+  typename Vec<C>::x8 v = *reinterpret_cast<const typename Vec<C>::x8*>(p);
+#pragma unroll
+  for (int i = 0; i < 8; i++) x[i] = (float)v[i];
+}
+template <> __device__ inline void load8<E4M3>(const uint8_t* p, float (&x)[8]) {
+  u32x2 v = *reinterpret_cast<const u32x2*>(p);
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(v[i], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(v[i], true);
+    x[4 * i] = lo[0], x[4 * i + 1] = lo[1], x[4 * i + 2] = hi[0], x[4 * i + 3] = hi[1];
+  }
+}
+
+__device__ inline float wave_max(float x) {
+#pragma unroll
+  for (int m = 32; m; m >>= 1) x = fmaxf(x, __shfl_xor(x, m));
+  return x;
+}
+__device__ inline float wave_sum(float x) {
+#pragma unroll
+  for (int m = 32; m; m >>= 1) x += __shfl_xor(x, m);
+  return x;
+}
+
+// Which request the packed row belongs to: the last i with cu[i] <= row, cu[requests] > row being known.
+__device__ inline int request_of(const int* cu, int requests, int row) {
+  int low = 0, high = requests;
+  while (high - low > 1) {
+    int mid = (low + high) >> 1;
+    if (cu[mid] <= row)
+      low = mid;
+    else
+      high = mid;
+  }
+  return low;
+}
+
+__device__ inline int clamp_int(int x, int low, int high) { return x < low ? low : (x > high ? high : x); }
+
+// Launches a kernel of one argument block, and says whether that worked.
+template <class Args> inline hipError_t launch(void (*kernel)(Args), dim3 grid, int threads, hipStream_t stream, const Args& args) {
+  void* list[] = {const_cast<Args*>(&args)};
+  return hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, dim3(threads), list, 0, stream);
+}
+
+// Calls F with the types that the arguments name.
+#define PAGED_DISPATCH(type, cache, F)                                                      \
+  ((cache) == Type::kE4M3 ? ((type) == Type::kBF16 ? F(BF16, E4M3) : F(FP16, E4M3))         \
+                          : ((type) == Type::kBF16 ? F(BF16, BF16) : F(FP16, FP16)))
+
+}  // namespace paged

@@ -1,0 +1,629 @@
+"""The paged key-value cache's operators against plain implementations in 64
+bits, on CPU tensors and, marked gpu, through the gfx950 kernels."""
+
+import math
+import random
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from beta9_amd.ops import paged  # noqa: E402
+
+DEVICES = [
+    "cpu",
+    pytest.param(
+        "cuda",
+        marks=[pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(), reason="needs MI355X")],
+    ),
+]
+TYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "e4m3": torch.float8_e4m3fn}
+both = pytest.mark.parametrize("device", DEVICES)
+
+
+def ints(values, device):
+    return torch.tensor(values, dtype=torch.int32, device=device)
+
+
+def cache_like(x, dtype, scale):
+    """x as an 8-bit cache or a plain one holds it."""
+    if dtype == torch.float8_e4m3fn:
+        return (x.float() / scale).clamp(-448, 448).to(dtype)
+    return x.to(dtype)
+
+
+def values_of(cache, scale=1.0):
+    return cache.cpu().to(torch.float64) * scale
+
+
+# -- plan and release -------------------------------------------------------
+
+
+def plan_oracle(tables, lens, new, stack, page, tokens):
+    """plan_step on lists. `stack`: the free pages, the top last."""
+    tables, stack = [list(t) for t in tables], list(stack)
+    slots, positions, cu, kv, after = [-1] * tokens, [0] * tokens, [0], [], []
+    wanted, available = 0, len(stack)
+    for r in range(len(lens)):
+        start, end = cu[-1], cu[-1] + new[r]
+        cu.append(end)
+        have, want = math.ceil(lens[r] / page), math.ceil((lens[r] + new[r]) / page)
+        ok = new[r] > 0 and want <= len(tables[r]) and end <= tokens
+        if ok:
+            wanted += want - have
+            ok = want == have or wanted <= available
+        if ok:
+            for c in range(have, want):
+                tables[r][c] = stack.pop()
+            for j in range(new[r]):
+                at = lens[r] + j
+                slots[start + j] = tables[r][at // page] * page + at % page
+                positions[start + j] = at
+        kv.append(lens[r] + new[r] if ok else 0)
+        after.append(lens[r] + new[r] if ok else lens[r])
+    return tables, slots, positions, cu, kv, after, len(stack)
+
+
+def plan_inputs(rng, requests, page, longest, most_new, width, spare):
+    lens = [rng.choice([0, 1, page - 1, page, page + 1, rng.randint(0, longest)]) for _ in range(requests)]
+    lens = [min(n, longest, width * page) for n in lens]
+    new = [rng.choice([0, 1, rng.randint(0, most_new)]) for _ in range(requests)]
+    held = sum(math.ceil(n / page) for n in lens)
+    pages = list(range(held + spare))
+    rng.shuffle(pages)
+    tables = []
+    for n in lens:
+        count = math.ceil(n / page)
+        tables.append([pages.pop() for _ in range(count)] + [-1] * (width - count))
+    return tables, lens, new, pages, held + spare
+
+
+@both
+@pytest.mark.parametrize(
+    "requests,page,longest,most_new,width,spare,short",
+    [
+        (1, 16, 40, 1, 4, 9, 0),
+        (5, 16, 100, 50, 10, 40, 0),
+        (33, 64, 500, 70, 9, 20, 0),  # too few pages for some
+        (257, 32, 200, 90, 8, 300, 0),  # rows that overflow
+        (700, 128, 900, 300, 12, 900, 0),
+        (4096, 16, 64, 20, 6, 9000, 0),
+        (9, 16, 50, 30, 8, 60, 25),  # fewer token rows than tokens
+        (3, 256, 1000, 5000, 30, 0, 0),  # no free page at all
+    ],
+)
+def test_plan_step(device, requests, page, longest, most_new, width, spare, short):
+    rng = random.Random(requests * 1000 + page)
+    tables, lens, new, stack, pool = plan_inputs(rng, requests, page, longest, most_new, width, spare)
+    tokens = max(0, sum(new) - short) + (3 if not short else 0)
+    want = plan_oracle(tables, lens, new, stack, page, tokens)
+    # rows of a wider tensor, so that their stride is not their width
+    wide = torch.full((requests, width + 3), -7, dtype=torch.int32, device=device)
+    t = wide[:, :width]
+    t.copy_(ints(tables, device))
+    free = ints(stack + [-1] * (pool - len(stack)), device)
+    count = ints([len(stack)], device)
+    for _ in range(2):  # a plan that is not stored can be made again
+        p = paged.plan_step(t, ints(lens, device), ints(new, device), free, count, page, tokens)
+        assert t.tolist() == want[0]
+        for got, expected in zip(p, want[1:6]):
+            assert got.dtype == torch.int32 and got.tolist() == expected
+        assert p.free_count.tolist() == [want[6]]
+    assert count.tolist() == [len(stack)] and (wide[:, width:] == -7).all()
+
+
+@both
+def test_plan_step_bounds_what_it_reads(device):
+    """Values that a caller's mistake leaves on the GPU stay inside the tensors."""
+    tables = ints([[0, 99], [-5, 1], [2, 3]], device)
+    p = paged.plan_step(
+        tables, ints([3, 2, 1000], device), ints([2, 1, 1], device), ints([4, 5, 6, 0, 0, 0, 0], device), ints([50], device), 16, 4
+    )
+    # row 1 holds a page that the pool does not have; row 2 is full
+    assert p.slots.tolist() == [3, 4, -1, -1]
+    assert p.cu_new.tolist() == [0, 2, 3, 4] and p.kv_lens.tolist() == [5, 3, 0] and p.lens.tolist() == [5, 3, 32]
+    assert p.free_count.tolist() == [7]
+    p = paged.plan_step(tables, ints([3, 2, -4], device), ints([-2, 0, 1], device), ints([4, 5], device), ints([-1], device), 16, 1)
+    assert p.slots.tolist() == [-1] and p.free_count.tolist() == [0] and p.lens.tolist() == [3, 2, 0]
+    p = paged.plan_step(tables, ints([3, 2, 1], device), ints([0, 0, 0], device), ints([4, 5], device), ints([1], device), 16, 0)
+    assert p.slots.shape == (0,) and p.kv_lens.tolist() == [0, 0, 0]
+
+
+@both
+@pytest.mark.parametrize("requests,page,longest", [(1, 16, 50), (40, 32, 300), (300, 64, 1000), (4096, 16, 40)])
+def test_release_pages(device, requests, page, longest):
+    rng = random.Random(requests)
+    tables, lens, _, stack, pool = plan_inputs(rng, requests, page, longest, 1, math.ceil(longest / page), 11)
+    done = [rng.random() < 0.5 for _ in range(requests)]
+    expected = list(stack)
+    for r in range(requests):
+        if done[r]:
+            expected += tables[r][: math.ceil(lens[r] / page)]
+    free = ints(stack + [-1] * (pool - len(stack)), device)
+    after, count = paged.release_pages(
+        ints(tables, device), ints(lens, device), torch.tensor(done, device=device), free, ints([len(stack)], device), page
+    )
+    assert count.tolist() == [len(expected)]
+    assert free.tolist() == expected + [-1] * (pool - len(expected))
+    assert after.tolist() == [0 if d else n for d, n in zip(done, lens)]
+
+
+@both
+def test_release_stays_inside_the_stack(device):
+    free = ints([7, 7, 7], device)
+    after, count = paged.release_pages(
+        ints([[1, 2], [5, 6]], device), ints([17, 900], device), torch.tensor([True, True], device=device), free, ints([2], device), 16
+    )
+    assert free.tolist() == [7, 7, 1] and count.tolist() == [3] and after.tolist() == [0, 0]
+
+
+# -- write ------------------------------------------------------------------
+
+
+@both
+@pytest.mark.parametrize("kind,cached", [("bf16", "bf16"), ("fp16", "fp16"), ("bf16", "e4m3"), ("fp16", "e4m3")])
+@pytest.mark.parametrize("tokens,heads,dim,page,offset", [(1, 1, 8, 16, 0), (37, 3, 80, 16, 0), (300, 8, 128, 64, 0), (65, 2, 64, 32, 1)])
+def test_write_kv(device, kind, cached, tokens, heads, dim, page, offset):
+    """Exactly the value, or the nearest e4m3, at each slot, and nothing else changed. offset 1: rows off the 16-byte grid."""
+    gen = torch.Generator().manual_seed(tokens)
+    fused = (torch.randn((tokens, 2 * heads + 1, dim + offset), generator=gen) * 3).to(TYPES[kind]).to(device)
+    k, v = fused[:, :heads, offset:], fused[:, heads : 2 * heads, offset:]
+    k[0, 0, :6] = torch.tensor([math.nan, math.inf, -math.inf, 60000.0, -60000.0, 0.0])
+    pages = tokens // page + 2
+    k_cache = torch.full((pages, heads, page, dim), 1.0).to(TYPES[cached]).to(device)
+    v_cache = k_cache.clone()
+    slots = torch.randperm(pages * page, generator=gen)[:tokens].to(torch.int32)
+    if tokens > 5:
+        slots[3], slots[4] = -1, pages * page  # skipped
+    scales = (0.03125, 0.5) if cached == "e4m3" else (1.0, 1.0)  # powers of two: the quotient is exact
+    before = values_of(k_cache)
+    paged.write_kv(k, v, k_cache, v_cache, slots.to(device), *scales)
+    for x, cache, scale in ((k, k_cache, scales[0]), (v, v_cache, scales[1])):
+        want = before.clone()
+        for t, slot in enumerate(slots.tolist()):
+            if 0 <= slot < pages * page:
+                want[slot // page, :, slot % page] = values_of(cache_like(x[t].cpu(), TYPES[cached], scale))
+        assert torch.equal(values_of(cache).nan_to_num(7.5), want.nan_to_num(7.5))
+        assert torch.equal(values_of(cache).isnan(), want.isnan())
+
+
+@both
+def test_write_kv_rounds_every_quotient_to_the_nearest(device):
+    """All finite bf16 values against the list of e4m3 values, by a scale that is no power of two."""
+    x = torch.arange(1 << 16, dtype=torch.int32).to(torch.int16).view(torch.bfloat16)
+    x = x[x.isfinite()]
+    x = torch.cat([x, x.new_zeros(-len(x) % 128)]).reshape(-1, 1, 128)
+    scale = 0.37
+    k_cache = torch.zeros((len(x) // 16 + 1, 1, 16, 128), device=device).to(torch.float8_e4m3fn)
+    v_cache = k_cache.clone()
+    paged.write_kv(x.to(device), x.to(device), k_cache, v_cache, torch.arange(len(x), dtype=torch.int32, device=device), scale, 1.0)
+    grid = torch.arange(256, dtype=torch.int32).to(torch.uint8).view(torch.float8_e4m3fn).double()
+    grid = grid[grid.isfinite()].unique()
+    quotient = (x.double().flatten() / scale).clamp(-448, 448)
+    got = values_of(k_cache).reshape(-1)[: quotient.numel()]
+    up = torch.searchsorted(grid, quotient).clamp(1, len(grid) - 1)
+    nearest = torch.minimum((grid[up] - quotient).abs(), (quotient - grid[up - 1]).abs())
+    # 1 / scale and its product with x are rounded to 32 bits, half a step each: a quotient that lies that near to the
+    # middle of two values may go to either
+    assert ((got - quotient).abs() <= nearest + quotient.abs() * 2 * 2**-24 * 1.01).all()
+
+
+# -- attention --------------------------------------------------------------
+
+
+def attention_oracle(q, k_cache, v_cache, tables, kv_lens, cu, scale, k_scale, v_scale):
+    """The formula in 64 bits, row by row, and for each result how far off it may be."""
+    kind = q.dtype
+    half = torch.finfo(kind).eps / 2
+    q, k_cache, v_cache = q.cpu().double(), values_of(k_cache, k_scale), values_of(v_cache, v_scale)
+    rows, heads, dim = q.shape
+    pages, kv_heads, page, _ = k_cache.shape
+    out, off = torch.zeros_like(q), torch.zeros_like(q)
+    for r, length in enumerate(kv_lens):
+        length = max(0, min(length, len(tables[r]) * page))
+        first, last = cu[r], min(cu[r + 1], rows)
+        at = torch.arange(length)
+        entry = torch.tensor(tables[r] + [0], dtype=torch.int64)[at // page]
+        known = (entry >= 0) & (entry < pages)
+        at, entry = at[known], entry[known]
+        for h in range(heads if last > first else 0):
+            k, v = k_cache[entry, h * kv_heads // heads, at % page], v_cache[entry, h * kv_heads // heads, at % page]
+            x = q[first:last, h]
+            sees = at[None] <= torch.arange(length - (cu[r + 1] - first), length + last - cu[r + 1])[:, None]
+            any_key = sees.any(1, keepdim=True)
+            s = ((x @ k.T) * scale).masked_fill(~sees, -math.inf)
+            w = torch.softmax(torch.where(any_key, s, 0.0), 1).masked_fill(~sees, 0.0)
+            out[first:last, h] = w @ v
+            # Each score is a sum of dim products in 32 bits: off by (dim + 4) half steps of its terms' sizes, and as
+            # much, relatively, is its exponential; numerator and denominator both. The exponent's argument in base 2
+            # is rounded once more, to half a step of its size. A probability may be rounded to the result's type
+            # before its product with v, the sums to 32 bits, the result to its type.
+            size = ((x.abs() @ k.abs().T) * abs(scale)).masked_fill(~sees, 0.0).amax(1, keepdim=True) if len(at) else 0.0
+            score = (dim + 4 + 2) * 2**-24 * size + 2**-22
+            sums = (len(at) + 8) * 2**-24
+            off[first:last, h] = half * out[first:last, h].abs() + (half + 2 * score + 2 * sums) * (w @ v.abs()) * (1 + half)
+            if kind == torch.float16:
+                off[first:last, h] += 2**-25  # half a step of its subnormals
+    return out, off
+
+
+def make_cache(gen, lens, heads, dim, page, kind, cached, device, holes=False):
+    """Tables over shuffled pages; every slot that no token holds is NaN, inf or the type's largest."""
+    counts = [math.ceil(n / page) for n in lens]
+    pages = sum(counts) + 2
+    order = torch.randperm(pages, generator=gen).tolist()
+    width = max(max(counts), 1) + 1
+    tables = [[order.pop() for _ in range(c)] + [123456789] * (width - c) for c in counts]
+    scales = (0.02, 0.015) if cached == "e4m3" else (1.0, 1.0)
+    made = []
+    for scale in scales:
+        x = torch.full((pages, heads, page, dim), math.nan)
+        x[..., 1::3] = 448 * scale if cached == "e4m3" else math.inf
+        for r, n in enumerate(lens):
+            for c in range(counts[r]):
+                m = min(page, n - c * page)
+                x[tables[r][c], :, :m] = torch.randn((heads, m, dim), generator=gen)
+        made.append(cache_like(x, TYPES[cached], scale) if cached == "e4m3" else x.to(TYPES[kind]))
+    if holes:
+        for row, entry in zip(tables, (-1, pages, 2**31 - 1, -(2**31))):
+            row[0] = entry
+    return made[0].to(device), made[1].to(device), tables, scales
+
+
+HEADS = [(1, 1), (4, 4), (8, 2), (5, 1), (20, 1), (6, 2)]
+KINDS = [("bf16", "bf16"), ("fp16", "fp16"), ("bf16", "e4m3"), ("fp16", "e4m3")]
+
+
+def check_attention(got, q, cache, lens, cu, scale=None):
+    k_cache, v_cache, tables, scales = cache
+    scale = q.shape[-1] ** -0.5 if scale is None else scale
+    want, off = attention_oracle(q, k_cache, v_cache, tables, lens, cu, scale, *scales)
+    assert got.dtype == q.dtype and got.shape == q.shape
+    far = (got.cpu().double() - want).abs()
+    assert (far <= off).all(), f"off by {far.max():.3g}, at most {float((far / off.clamp(min=1e-30)).max()):.3g} of what is allowed"
+
+
+def run_decode(q, cache, lens, **more):
+    k_cache, v_cache, tables, scales = cache
+    d = q.device
+    return paged.decode_attention(q, k_cache, v_cache, ints(tables, d), ints(lens, d), k_scale=scales[0], v_scale=scales[1], **more)
+
+
+def run_prompt(q, cache, lens, cu, **more):
+    k_cache, v_cache, tables, scales = cache
+    d = q.device
+    return paged.prompt_attention(
+        q, k_cache, v_cache, ints(tables, d), ints(lens, d), ints(cu, d), k_scale=scales[0], v_scale=scales[1], **more
+    )
+
+
+@both
+@pytest.mark.parametrize("kind,cached", KINDS)
+@pytest.mark.parametrize("dim", [8, 64, 80, 128, 256])
+@pytest.mark.parametrize("heads,kv_heads", HEADS)
+def test_decode_attention(device, kind, cached, dim, heads, kv_heads):
+    page = {8: 16, 64: 16, 80: 64, 128: 32, 256: 128}[dim]
+    gen = torch.Generator().manual_seed(heads * dim)
+    lens = [0, 1, 2, 31, 32, 33, 64, 127, 0, 129, 257, 300]
+    cache = make_cache(gen, lens, kv_heads, dim, page, kind, cached, device)
+    q = torch.randn((len(lens), heads, dim), generator=gen).to(TYPES[kind]).to(device)
+    got = run_decode(q, cache, lens)
+    check_attention(got, q, cache, lens, list(range(len(lens) + 1)))
+    assert (got[0] == 0).all() and (got[8] == 0).all()
+
+
+@both
+@pytest.mark.parametrize("kind,cached", KINDS)
+@pytest.mark.parametrize("lens", [[5000], [1, 2049, 7, 4100], [640] * 40])
+def test_decode_attention_over_long_rows(device, kind, cached, lens):
+    gen = torch.Generator().manual_seed(len(lens))
+    cache = make_cache(gen, lens, 2, 64, 64, kind, cached, device)
+    q = (torch.randn((len(lens), 4, 64), generator=gen) * 2).to(TYPES[kind]).to(device)
+    check_attention(run_decode(q, cache, lens), q, cache, lens, list(range(len(lens) + 1)))
+
+
+@both
+@pytest.mark.parametrize("kind,cached", KINDS)
+@pytest.mark.parametrize("dim", [8, 64, 80, 128, 256])
+@pytest.mark.parametrize("heads,kv_heads", HEADS)
+def test_prompt_attention(device, kind, cached, dim, heads, kv_heads):
+    page = {8: 16, 64: 16, 80: 64, 128: 32, 256: 128}[dim]
+    gen = torch.Generator().manual_seed(heads * dim + 1)
+    new = [1, 0, 3, 40, 0, 1, 17]
+    held = [0, 5, 60, 0, 0, 130, 33]
+    lens = [h + n for h, n in zip(held, new)]
+    cu = [0]
+    for n in new:
+        cu.append(cu[-1] + n)
+    cache = make_cache(gen, lens, kv_heads, dim, page, kind, cached, device)
+    q = torch.randn((cu[-1], heads, dim), generator=gen).to(TYPES[kind]).to(device)
+    check_attention(run_prompt(q, cache, lens, cu), q, cache, lens, cu)
+
+
+@both
+@pytest.mark.parametrize("kind,cached", KINDS)
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 128)])
+def test_prompt_attention_over_many_tiles(device, kind, cached, dim, page):
+    gen = torch.Generator().manual_seed(dim)
+    new, held = [150, 2, 333], [1, 500, 0]
+    lens = [h + n for h, n in zip(held, new)]
+    cu = [0, 150, 152, 485]
+    cache = make_cache(gen, lens, 2, dim, page, kind, cached, device)
+    q = (torch.randn((cu[-1], 4, dim), generator=gen) * 2).to(TYPES[kind]).to(device)
+    check_attention(run_prompt(q, cache, lens, cu), q, cache, lens, cu)
+
+
+@both
+@pytest.mark.parametrize("dim", [80, 64, 128])
+def test_attention_with_entries_that_name_no_page(device, dim):
+    """Their tokens count as absent, whatever the other pages hold."""
+    gen = torch.Generator().manual_seed(3)
+    lens = [20, 70, 33, 16, 40]
+    cache = make_cache(gen, lens, 1, dim, 16, "bf16", "bf16", device, holes=True)
+    q = torch.randn((5, 2, dim), generator=gen).to(torch.bfloat16).to(device)
+    got = run_decode(q, cache, lens)
+    check_attention(got, q, cache, lens, list(range(6)))
+    assert (got[3] == 0).all()
+    cu = [0, 20, 50, 60, 70, 72]
+    q = torch.randn((72, 2, dim), generator=gen).to(torch.bfloat16).to(device)
+    check_attention(run_prompt(q, cache, lens, cu), q, cache, lens, cu)
+
+
+@both
+@pytest.mark.parametrize("dim", [80, 64, 128])
+def test_lengths_past_the_table_end_with_it(device, dim):
+    gen = torch.Generator().manual_seed(4)
+    k_cache, v_cache, tables, scales = make_cache(gen, [32, 32], 1, dim, 16, "bf16", "bf16", device)
+    cache = (k_cache, v_cache, [t[:2] for t in tables], scales)
+    q = torch.randn((2, 1, dim), generator=gen).to(torch.bfloat16).to(device)
+    got = run_decode(q, cache, [2**31 - 1, -3])
+    check_attention(got, q, cache, [32, 0], [0, 1, 2])
+    # more new rows than tokens: the first rows see nothing
+    q = torch.randn((40, 1, dim), generator=gen).to(torch.bfloat16).to(device)
+    got = run_prompt(q, cache, [32, 0], [0, 40, 40])
+    check_attention(got, q, cache, [32, 0], [0, 40, 40])
+    assert (got[:8] == 0).all()
+
+
+@both
+@pytest.mark.parametrize("dim", [80, 64, 128])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_later_tokens_do_not_reach_earlier_rows(device, dim, bad):
+    """A value or key that is not finite changes the rows that see it and no others."""
+    gen = torch.Generator().manual_seed(5)
+    k_cache, v_cache, tables, scales = make_cache(gen, [200], 2, dim, 16, "bf16", "bf16", device)
+    q = torch.randn((200, 4, dim), generator=gen).to(torch.bfloat16).to(device)
+    for which in (0, 1):
+        caches = [k_cache.clone(), v_cache.clone()]
+        caches[which][tables[0][150 // 16], 1, 150 % 16, 7] = bad
+        got = run_prompt(q, (*caches, tables, scales), [200], [0, 200])
+        cache = (k_cache, v_cache, tables, scales)
+        check_attention(got[:150], q[:150], cache, [150], [0, 150])
+        check_attention(got[:, :2], q[:, :2], (k_cache[:, :1], v_cache[:, :1], tables, scales), [200], [0, 200])
+        touched = got[150:, 2:].isfinite() if which == 0 else got[150:, 2:, 7].isfinite()
+        if which == 0 and bad == math.inf:
+            # q * inf is +inf (no value for the row: inf - inf) or -inf (the token's weight is 0)
+            negative = q[150:, 2:, 7] < 0
+            assert (touched == negative[..., None]).all()
+        else:
+            assert not touched.any()
+        if which == 1:
+            rest = [d for d in range(dim) if d != 7]
+            want, off = attention_oracle(q, k_cache, v_cache, tables, [200], [0, 200], dim**-0.5, *scales)
+            assert ((got.cpu().double() - want).abs() <= off)[:, :, rest].all()
+
+
+@both
+@pytest.mark.parametrize("dim", [80, 64, 128])
+def test_scores_far_apart(device, dim):
+    """Scores of thousands, all equal scores, and a maximum that comes first or last."""
+    gen = torch.Generator().manual_seed(6)
+    cache = make_cache(gen, [300, 300, 300], 1, dim, 64, "fp16", "fp16", device)
+    q = torch.randn((3, 2, dim), generator=gen).half().to(device)
+    q[0] *= 200
+    q[1] = 0
+    tables = cache[2]
+    cache[0][tables[2][0], 0, 0] = q[2, 0] * 4
+    cache[0][tables[2][4], 0, 300 - 257] = q[2, 1] * 4
+    check_attention(run_decode(q, cache, [300] * 3), q, cache, [300] * 3, [0, 1, 2, 3])
+    check_attention(run_decode(q, cache, [300] * 3, scale=-0.5), q, cache, [300] * 3, [0, 1, 2, 3], scale=-0.5)
+    check_attention(run_prompt(q, cache, [300] * 3, [0, 1, 2, 3], scale=0.01), q, cache, [300] * 3, [0, 1, 2, 3], scale=0.01)
+
+
+@both
+@pytest.mark.parametrize("dim", [80, 64, 128])
+def test_strided_queries_and_given_results(device, dim):
+    gen = torch.Generator().manual_seed(7)
+    lens, cu = [90, 0, 33], [0, 50, 50, 60]
+    cache = make_cache(gen, lens, 2, dim, 16, "bf16", "bf16", device)
+    for offset in (0, 1, 8):  # 1: rows off the 16-byte grid
+        fused = torch.randn((64, 9, dim + offset), generator=gen).to(torch.bfloat16).to(device)
+        q = fused[:, 2:6, offset:]
+        out = torch.full((64, 4, dim), 5.0, dtype=torch.bfloat16, device=device)
+        got = run_prompt(q, cache, lens, cu, out=out)
+        assert got.data_ptr() == out.data_ptr() and (out[60:] == 5).all()
+        check_attention(out[:60], q[:60], cache, lens, cu)
+        fresh = run_prompt(q, cache, lens, cu)
+        assert (fresh[60:] == 0).all() and torch.equal(fresh[:60], out[:60])
+        q = q.transpose(0, 1)[:, :3].transpose(0, 1)
+        out = torch.full((3, 4, dim), 5.0, dtype=torch.bfloat16, device=device)
+        run_decode(q, cache, lens, out=out)
+        check_attention(out, q, cache, lens, [0, 1, 2, 3])
+
+
+@both
+def test_empty_calls(device):
+    cache = torch.zeros((2, 2, 16, 64), dtype=torch.bfloat16, device=device)
+    none = torch.zeros((0, 4, 64), dtype=torch.bfloat16, device=device)
+    tables, zero = ints([[0, 1]], device), ints([0], device)
+    assert paged.decode_attention(none, cache, cache, tables[:0], zero[:0]).shape == (0, 4, 64)
+    assert paged.prompt_attention(none, cache, cache, tables, zero, ints([0, 0], device)).shape == (0, 4, 64)
+    paged.write_kv(none[:, :2], none[:, :2], cache, cache.clone(), zero[:0])
+    q = torch.ones((3, 4, 64), dtype=torch.bfloat16, device=device)
+    assert (paged.prompt_attention(q, cache, cache, tables[:0], zero[:0], zero) == 0).all()
+
+
+# -- refusals ---------------------------------------------------------------
+
+
+def good(device):
+    bf16 = dict(dtype=torch.bfloat16, device=device)
+    return dict(
+        q=torch.zeros((3, 4, 64), **bf16),
+        k_cache=torch.zeros((5, 2, 16, 64), **bf16),
+        v_cache=torch.zeros((5, 2, 16, 64), **bf16),
+        tables=torch.zeros((3, 2), dtype=torch.int32, device=device),
+        kv_lens=torch.zeros(3, dtype=torch.int32, device=device),
+    )
+
+
+@both
+@pytest.mark.parametrize(
+    "change,error",
+    [
+        (dict(q=lambda x: x.int()), TypeError),
+        (dict(q=lambda x: x[0]), ValueError),
+        (dict(q=lambda x: x[:2]), ValueError),
+        (dict(q=lambda x: x[:, :3]), ValueError),
+        (dict(q=lambda x: x[..., :32]), ValueError),
+        (dict(q=lambda x: x.repeat(1, 1, 2)[..., ::2]), ValueError),
+        (dict(q=lambda x: x.requires_grad_()), RuntimeError),
+        (dict(k_cache=lambda x: x.half()), TypeError),
+        (dict(v_cache=lambda x: x.to(torch.float8_e4m3fn)), TypeError),
+        (dict(k_cache=lambda x: x[:4]), ValueError),
+        (dict(k_cache=lambda x: x.transpose(1, 2), v_cache=lambda x: x.transpose(1, 2)), ValueError),
+        (dict(k_cache=lambda x: x[:, :, :10].contiguous(), v_cache=lambda x: x[:, :, :10].contiguous()), ValueError),
+        (dict(k_cache=lambda x: x[0], v_cache=lambda x: x[0]), ValueError),
+        (dict(k_cache=lambda x: x[:0], v_cache=lambda x: x[:0]), ValueError),
+        (dict(tables=lambda x: x.long()), TypeError),
+        (dict(tables=lambda x: x[0]), ValueError),
+        (dict(tables=lambda x: x[:, :0]), ValueError),
+        (dict(tables=lambda x: x.t().contiguous().t()), ValueError),
+        (dict(tables=lambda x: x[:2]), ValueError),
+        (dict(kv_lens=lambda x: x.float()), TypeError),
+        (dict(kv_lens=lambda x: x[:2]), ValueError),
+        (dict(kv_lens=lambda x: x.repeat(2)[::2]), ValueError),
+        (dict(scale=math.nan), ValueError),
+        (dict(k_scale=2.0), ValueError),
+        (dict(v_scale=0.0), ValueError),
+        (dict(k_scale=math.inf), ValueError),
+        (dict(out=lambda q: q.clone().half()), TypeError),
+        (dict(out=lambda q: q), ValueError),
+        (dict(out=lambda q: q.clone()[:, :2]), ValueError),
+        (dict(out=lambda q: torch.cat([q, q], 1)[:, :4]), ValueError),
+    ],
+)
+def test_attention_refusals(device, change, error):
+    args, more = good(device), {}
+    for name, f in change.items():
+        if name in args:
+            args[name] = f(args[name])
+        else:
+            more[name] = f(args["q"]) if callable(f) else f
+    with pytest.raises(error):
+        paged.decode_attention(*args.values(), **more)
+    cu = torch.zeros(4, dtype=torch.int32, device=device)
+    if set(change) != {"q"} or error is not ValueError or args["q"].shape[1:] != (4, 64) or args["q"].stride(2) != 1:
+        with pytest.raises(error):
+            paged.prompt_attention(*args.values(), cu, **more)
+    args = good(device)
+    for bad, e in ((cu[:3], ValueError), (cu.long(), TypeError), (cu.repeat(2)[::2], ValueError)):
+        with pytest.raises(e):
+            paged.prompt_attention(*args.values(), bad)
+
+
+@both
+def test_head_dims_are_refused_that_no_kernel_takes(device):
+    for dim in (4, 12, 264):
+        q = torch.zeros((1, 1, dim), dtype=torch.bfloat16, device=device)
+        cache = torch.zeros((1, 1, 16, dim), dtype=torch.bfloat16, device=device)
+        with pytest.raises(ValueError):
+            paged.decode_attention(q, cache, cache, ints([[0]], device), ints([0], device))
+        with pytest.raises(ValueError):
+            paged.write_kv(q, q, cache, cache, ints([0], device))
+
+
+@both
+@pytest.mark.parametrize(
+    "change,error",
+    [
+        (dict(k=lambda x: x.int()), TypeError),
+        (dict(v=lambda x: x.half()), TypeError),
+        (dict(k=lambda x: x[:, :1]), ValueError),
+        (dict(k=lambda x: x[:, :1], v=lambda x: x[:, :1]), ValueError),
+        (dict(k=lambda x: x.repeat(1, 1, 2)[..., ::2]), ValueError),
+        (dict(slots=lambda x: x.long()), TypeError),
+        (dict(slots=lambda x: x[:1]), ValueError),
+        (dict(slots=lambda x: x[None]), ValueError),
+        (dict(k_cache=lambda x: x[:, :, :, :32]), ValueError),
+        (dict(k_scale=0.5), ValueError),
+        (dict(v_scale=-1.0), ValueError),
+        (dict(k=lambda x: x.requires_grad_()), RuntimeError),
+    ],
+)
+def test_write_refusals(device, change, error):
+    bf16 = dict(dtype=torch.bfloat16, device=device)
+    args = dict(k=torch.zeros((2, 2, 64), **bf16), v=torch.zeros((2, 2, 64), **bf16))
+    args |= dict(k_cache=torch.zeros((5, 2, 16, 64), **bf16), v_cache=torch.zeros((5, 2, 16, 64), **bf16), slots=ints([0, 1], device))
+    for name, f in change.items():
+        args[name] = f(args[name]) if callable(f) else f
+    with pytest.raises(error):
+        paged.write_kv(**args)
+
+
+@both
+@pytest.mark.parametrize(
+    "change,error",
+    [
+        (dict(page_size=24), ValueError),
+        (dict(page_size=8), ValueError),
+        (dict(page_size=512), ValueError),
+        (dict(num_tokens=-1), ValueError),
+        (dict(tables=lambda x: x.float()), TypeError),
+        (dict(tables=lambda x: x[:0]), ValueError),
+        (dict(tables=lambda x: x.repeat(3000, 1)), ValueError),
+        (dict(lens=lambda x: x[:1]), ValueError),
+        (dict(lens=lambda x: x.long()), TypeError),
+        (dict(new_lens=lambda x: x[:1]), ValueError),
+        (dict(new_lens=lambda x: x.long()), TypeError),
+        (dict(free_pages=lambda x: x[None]), ValueError),
+        (dict(free_pages=lambda x: x.repeat(2)[::2]), ValueError),
+        (dict(free_count=lambda x: x.repeat(2)), ValueError),
+        (dict(free_count=lambda x: x.float()), TypeError),
+    ],
+)
+def test_plan_refusals(device, change, error):
+    args = dict(tables=ints([[0, 1], [2, 3]], device), lens=ints([1, 1], device), new_lens=ints([1, 1], device))
+    args |= dict(free_pages=ints([4, 5], device), free_count=ints([2], device), page_size=16, num_tokens=2)
+    for name, f in change.items():
+        args[name] = f(args[name]) if callable(f) else f
+    with pytest.raises(error):
+        paged.plan_step(**args)
+    if "new_lens" in change or "num_tokens" in change:
+        return
+    args["done"] = torch.zeros(2, dtype=torch.bool, device=device)
+    del args["new_lens"], args["num_tokens"]
+    with pytest.raises(error):
+        paged.release_pages(**args)
+
+
+@both
+def test_release_refusals(device):
+    tables, lens = ints([[0, 1], [2, 3]], device), ints([1, 1], device)
+    free, count = ints([4, 5], device), ints([1], device)
+    for done, error in ((ints([0, 0], device), TypeError), (torch.zeros(3, dtype=torch.bool, device=device), ValueError)):
+        with pytest.raises(error):
+            paged.release_pages(tables, lens, done, free, count, 16)
+
+
+@pytest.mark.gpu
+@pytest.mark.skipif(not torch.cuda.is_available(), reason="needs MI355X")
+def test_tensors_of_two_devices_are_refused():
+    args = good("cuda")
+    for name in ("k_cache", "v_cache", "tables", "kv_lens"):
+        with pytest.raises(ValueError):
+            paged.decode_attention(**{**args, name: args[name].cpu()})
+    with pytest.raises((ValueError, TypeError)):
+        paged.decode_attention(**{**args, "q": args["q"].cpu()})
+    with pytest.raises(TypeError):
+        paged.decode_attention(**{n: x.float() if x.is_floating_point() else x for n, x in args.items()})
