@@ -70,7 +70,7 @@ Type check_caches(const Tensor& k, const Tensor& v, const Tensor& like, Type typ
 void check_table(const Tensor& tables, const Tensor& like, int64_t page_size) {
   check_ints(tables, like, 2, "tables");
   REQUIRE(tables.size(0) <= paged::kMaxRequests, "at most ", paged::kMaxRequests, " requests, got ", tables.size(0));
-  REQUIRE(tables.size(1) >= 1 && tables.size(1) * page_size < (1LL << 31), "a table row must name at least 1 and fewer than 2^31 slots");
+  REQUIRE(tables.size(1) >= 1 && tables.size(1) * page_size <= (1LL << 30), "a table row must name at least 1 and at most 2^30 slots");
 }
 
 void check_scale(double x, const char* name) { REQUIRE(std::isfinite(x) && x > 0, name, " must be a positive number, is ", x); }
@@ -170,7 +170,7 @@ Tensor attend(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, con
   REQUIRE(q.dim() == 3 && q.size(2) == dim, "q must be [rows, heads, ", dim, "] for this cache");
   REQUIRE(q.size(1) >= 1 && q.size(1) % kv_heads == 0, "q's ", q.size(1), " heads must be a multiple of the cache's ", kv_heads);
   REQUIRE(q.numel() == 0 || q.stride(2) == 1, "q must have no gaps along the head dim");
-  REQUIRE(q.size(0) * q.size(1) < (1LL << 31), "too many rows");
+  REQUIRE(q.size(0) < (1LL << 31) / q.size(1) && q.size(1) <= 65535, "too many rows or heads");
   check_table(tables, q, page_size);
   check_ints(kv_lens, q, 1, "kv_lens");
   int64_t requests = tables.size(0);
@@ -206,6 +206,13 @@ Tensor attend(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, con
   a.width = (int)tables.size(1), a.pages = (int)k_cache.size(0);
   a.score_scale = (float)(scale * k_scale * kLog2E), a.value_scale = (float)v_scale;
   a.clear_rest = out_given ? 0 : 1;
+  if (!cu_new && paged::decode_takes(a)) {
+    Tensor workspace;
+    int64_t floats = paged::decode_workspace(a);
+    if (floats) workspace = at::empty({floats}, q.options().dtype(at::kFloat));
+    launched(paged::launch_decode(a, floats ? workspace.data_ptr<float>() : nullptr, current_stream()), "decode_attention");
+    return out;
+  }
   launched(paged::launch_attend_rows(a, current_stream()), cu_new ? "prompt_attention" : "decode_attention");
   return out;
 }

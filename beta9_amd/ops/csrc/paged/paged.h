@@ -80,6 +80,10 @@ struct AttendArgs {
 hipError_t launch_plan(const PlanArgs& a, hipStream_t stream);
 hipError_t launch_release(const ReleaseArgs& a, hipStream_t stream);
 hipError_t launch_write(const WriteArgs& a, hipStream_t stream);
+// For head dims of 64 and 128; workspace: as many floats as decode_workspace says.
+bool decode_takes(const AttendArgs& a);
+int64_t decode_workspace(const AttendArgs& a);
+hipError_t launch_decode(const AttendArgs& a, float* workspace, hipStream_t stream);
 hipError_t launch_attend_rows(const AttendArgs& a, hipStream_t stream);
 
 }  // namespace paged

@@ -318,8 +318,8 @@ def _check_table(tables: torch.Tensor, like: torch.Tensor, page_size: int) -> No
     _check_ints(tables, like, 2, "tables")
     _require(tables.shape[0] <= MAX_REQUESTS, f"at most {MAX_REQUESTS} requests, got {tables.shape[0]}")
     _require(
-        tables.shape[1] >= 1 and tables.shape[1] * page_size < 2**31,
-        "a table row must name at least 1 and fewer than 2^31 slots",
+        tables.shape[1] >= 1 and tables.shape[1] * page_size <= 2**30,
+        "a table row must name at least 1 and at most 2^30 slots",
     )
 
 
@@ -460,6 +460,7 @@ def _attend_plain(q, k_cache, v_cache, tables, kv_lens, cu_new, scale, k_scale, 
     pages, kv_heads, page_size, dim = k_cache.shape
     _require(q.dim() == 3 and q.shape[2] == dim, f"q must be [rows, heads, {dim}] for this cache")
     rows, heads = q.shape[:2]
+    _require(heads <= 65535, "too many rows or heads")
     _require(
         heads >= 1 and heads % kv_heads == 0, f"q's {heads} heads must be a multiple of the cache's {kv_heads}"
     )
