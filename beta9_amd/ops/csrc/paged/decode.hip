@@ -51,8 +51,9 @@ __device__ inline Share share_of(const SplitArgs& s, int item, int request_wante
     int l = i < a.requests ? a.kv_lens[i] : 0;
     return (int)max((int64_t)0, min((int64_t)l, room));
   };
-  int64_t total = 0;
-  for (int i = lane; i < a.requests; i += 64) total += length(i);
+  int mine = length(lane);  // the first 64 requests' lengths stay here for both passes
+  int64_t total = mine;
+  for (int i = lane + 64; i < a.requests; i += 64) total += length(i);
 #pragma unroll
   for (int m = 32; m; m >>= 1) total += __shfl_xor((long long)total, m);
   int64_t even = (total + s.target - 1) / s.target;
@@ -60,7 +61,7 @@ __device__ inline Share share_of(const SplitArgs& s, int item, int request_wante
   uint32_t chunk = (uint32_t)min((int64_t)1 << 31, max((int64_t)s.least, (even + kStep - 1) / kStep * kStep));
   int before = 0;
   for (int first = 0; first < a.requests; first += 64) {
-    int i = first + lane, l = length(i);
+    int i = first + lane, l = first ? length(i) : mine;
     // a request without keys has one chunk all the same: its zeros
     int n = i < a.requests ? max(1, (int)(((uint32_t)l + chunk - 1u) / chunk)) : 0;
     int up = n;
@@ -132,7 +133,7 @@ template <class X, class C, int D> struct Decode {
 };
 
 template <class X, class C, int D>
-__global__ __launch_bounds__(kWaves * 64, 2) void split_kernel(SplitArgs s) {
+__global__ __launch_bounds__(kWaves * 64, 4) void split_kernel(SplitArgs s) {
   typedef Decode<X, C, D> K;
   typedef typename K::Half8 Half8;
   const AttendArgs& a = s.a;
@@ -222,12 +223,15 @@ __global__ __launch_bounds__(kWaves * 64, 2) void split_kernel(SplitArgs s) {
       for (int i = 0; i < K::kPer; i++) acc[i] *= alpha;
     }
     float from = (m == kMinusInf ? 0.f : m) - K::kBias;
-    Half8 p;
+    // The probabilities in two parts, what rounding to 16 bits leaves behind being the second: as exact as in 32 bits
+    // for a second matrix product, which costs nothing next to the loads.
+    Half8 p, rest;
 #pragma unroll
     for (int j = 0; j < 8; j++) {
       float y = __builtin_amdgcn_exp2f(x[j] - from);
       l += y;
-      p[j] = (typename X::T)y;  // rounded for the matrix product; the sum l is not
+      p[j] = (typename X::T)y;
+      rest[j] = (typename X::T)(y - (float)p[j]);
     }
     // the lane's 8 keys by kPer dims, dim by dim
     uint32_t w[8][K::kPer / 2];
@@ -240,41 +244,41 @@ __global__ __launch_bounds__(kWaves * 64, 2) void split_kernel(SplitArgs s) {
         else
           w[j][i] = t.v[j][i];
       }
+    // An infinite value makes its sums infinite; a second part of zero or of another sign would make them NaN. (e4m3 has
+    // no infinities.)
+    bool finite = true;
+    if constexpr (!K::kNarrow) {
+      typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+      u16x2 most = {};
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+#pragma unroll
+        for (int i = 0; i < K::kPer / 2; i++) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, w[j][i] & 0x7fff7fffu));
+      finite = !__any(max(most[0], most[1]) >= (__is_same(X, BF16) ? 0x7f80 : 0x7c00));
+    }
 #pragma unroll
     for (int i = 0; i < K::kPer; i++) {
-      u32x4 column;
+      u32x4 x;
 #pragma unroll
       for (int j = 0; j < 4; j++)
-        column[j] = __builtin_amdgcn_perm(w[2 * j + 1][i >> 1], w[2 * j][i >> 1], i & 1 ? 0x07060302u : 0x05040100u);
-      acc[i] = K::product(__builtin_bit_cast(Half8, column), p, acc[i]);
+        x[j] = __builtin_amdgcn_perm(w[2 * j + 1][i >> 1], w[2 * j][i >> 1], i & 1 ? 0x07060302u : 0x05040100u);
+      acc[i] = K::product(__builtin_bit_cast(Half8, x), p, acc[i]);
+      if (finite) acc[i] = K::product(__builtin_bit_cast(Half8, x), rest, acc[i]);
     }
   };
 
-  // Two tiles of registers: one is computed with while the other is on its way, the entries of the table a tile ahead
-  // of that.
+  // One tile of registers, the table's entries a tile ahead: 126 registers, so that four waves share a SIMD and one
+  // computes while the others' loads are on their way. A second tile (221 registers, two waves) measured 33.4 us
+  // instead of 31.6 on 32 ragged rows up to 2048, 98.9 instead of 98.5 on one of 131071 (bf16, 8 kv heads of 128).
   constexpr int kStride = kWaves * kTile;
   int base = first + wave * kTile;
   if (base < last) {
-    typename K::Tile even, odd;
-    fetch(even, base, entry_of(base + k_key), entry_of(base + v_key));
-    int k_page = entry_of(base + kStride + k_key), v_page = entry_of(base + kStride + v_key);
-    while (true) {
-      bool more = base + kStride < last;
-      if (more) {
-        fetch(odd, base + kStride, k_page, v_page);
-        k_page = entry_of(base + 2 * kStride + k_key), v_page = entry_of(base + 2 * kStride + v_key);
-      }
-      use(even, base);
-      base += kStride;
-      if (!more) break;
-      more = base + kStride < last;
-      if (more) {
-        fetch(even, base + kStride, k_page, v_page);
-        k_page = entry_of(base + 2 * kStride + k_key), v_page = entry_of(base + 2 * kStride + v_key);
-      }
-      use(odd, base);
-      base += kStride;
-      if (!more) break;
+    typename K::Tile t;
+    int k_page = entry_of(base + k_key), v_page = entry_of(base + v_key);
+    for (; base < last; base += kStride) {
+      fetch(t, base, k_page, v_page);
+      k_page = entry_of(base + kStride + k_key), v_page = entry_of(base + kStride + v_key);
+      use(t, base);
     }
   }
 
@@ -312,55 +316,89 @@ __global__ __launch_bounds__(kWaves * 64, 2) void split_kernel(SplitArgs s) {
   }
 }
 
-// Joins the chunks of one request and head: the waves take chunks in turn, a lane D / 64 dims.
-template <class X, int D>
+// Joins a request's chunks, for kJoin heads a workgroup: D / 4 threads a head, the rest of the 256 take chunks in turn,
+// four on their way at a time.
+template <class X, int D, int kJoin>
 __global__ __launch_bounds__(kWaves * 64) void join_kernel(SplitArgs s) {
   const AttendArgs& a = s.a;
-  __shared__ float o_lds[kWaves][D];
-  __shared__ float l_lds[kWaves];
+  constexpr int kLanes = D / 4, kSlots = kWaves * 64 / (kLanes * kJoin), kAhead = 4;
+  __shared__ float o_lds[kSlots][kJoin][D];
+  __shared__ float m_lds[kSlots][kJoin], l_lds[kSlots][kJoin];
   Share share = share_of(s, 0, blockIdx.x);
   if (share.count <= 1) return;
-  constexpr int kPer = D / 64;
-  int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, head = blockIdx.y;
-  int64_t first = share.index;
-  float top = kMinusInf;
-  for (int i = lane; i < share.count; i += 64) top = fmaxf(top, s.stats[2 * ((first + i) * a.heads + head)]);
-  top = wave_max(top);
-  float sum = 0.f, o[kPer] = {};
-  for (int i = wave; i < share.count; i += kWaves) {
-    int64_t at = (first + i) * a.heads + head;
-    float f = top == kMinusInf ? 0.f : __builtin_amdgcn_exp2f(s.stats[2 * at] - top);
-    sum += f * s.stats[2 * at + 1];
+  int dim = (threadIdx.x % kLanes) * 4, at = threadIdx.x / kLanes, here = at % kJoin, slot = at / kJoin;
+  int head = blockIdx.y * kJoin + here;
+  bool real = head < a.heads;
+  int64_t first = (int64_t)share.index * a.heads + (real ? head : 0);
+  float m = kMinusInf, l = 0.f;
+  f32x4 o = {};
+  for (int i = slot; i < share.count; i += kAhead * kSlots) {
+    f32x4 x[kAhead];
+    f32x2 stat[kAhead];
 #pragma unroll
-    for (int d = 0; d < kPer; d++) o[d] += f * s.part[at * D + lane * kPer + d];
+    for (int j = 0; j < kAhead; j++) {
+      int64_t from = first + (int64_t)min(i + j * kSlots, share.count - 1) * a.heads;
+      x[j] = *reinterpret_cast<const f32x4*>(s.part + from * D + dim);
+      stat[j] = *reinterpret_cast<const f32x2*>(s.stats + 2 * from);
+      if (i + j * kSlots >= share.count) stat[j] = f32x2{kMinusInf, 0.f}, x[j] = f32x4{};
+    }
+    float top = m;
+#pragma unroll
+    for (int j = 0; j < kAhead; j++) top = fmaxf(top, stat[j][0]);
+    if (top == kMinusInf) continue;
+    float f = __builtin_amdgcn_exp2f(m - top);
+    m = top, l *= f, o *= f;
+#pragma unroll
+    for (int j = 0; j < kAhead; j++) {
+      f = __builtin_amdgcn_exp2f(stat[j][0] - top);
+      l += f * stat[j][1], o += f * x[j];
+    }
   }
-#pragma unroll
-  for (int d = 0; d < kPer; d++) o_lds[wave][lane * kPer + d] = o[d];
-  if (lane == 0) l_lds[wave] = sum;
+  *reinterpret_cast<f32x4*>(&o_lds[slot][here][dim]) = o;
+  if (dim == 0) m_lds[slot][here] = m, l_lds[slot][here] = l;
   __syncthreads();
-  if (threadIdx.x >= D) return;
-  float l = 0.f, x = 0.f;
+  if (slot || !real) return;
+  float top = m;
 #pragma unroll
-  for (int w = 0; w < kWaves; w++) l += l_lds[w], x += o_lds[w][threadIdx.x];
-  typename X::T* out = (typename X::T*)a.out + share.request * a.out_row + head * a.out_head;
-  out[threadIdx.x] = (typename X::T)(l == 0.f ? 0.f : x * (a.value_scale / l));
+  for (int w = 1; w < kSlots; w++) top = fmaxf(top, m_lds[w][here]);
+  float f = top == kMinusInf ? 0.f : __builtin_amdgcn_exp2f(m - top);
+  l *= f, o *= f;
+#pragma unroll
+  for (int w = 1; w < kSlots; w++) {
+    f = top == kMinusInf ? 0.f : __builtin_amdgcn_exp2f(m_lds[w][here] - top);
+    l += f * l_lds[w][here], o += f * *reinterpret_cast<const f32x4*>(&o_lds[w][here][dim]);
+  }
+  typename X::T* out = (typename X::T*)a.out + share.request * a.out_row + head * a.out_head + dim;
+  f = l == 0.f ? 0.f : a.value_scale / l;
+#pragma unroll
+  for (int i = 0; i < 4; i++) out[i] = (typename X::T)(l == 0.f ? 0.f : o[i] * f);
 }
 
-constexpr int kWorkgroups = 2048;
+// Keys of a chunk at least: shorter ones spend their time on starting and joining.
 constexpr int kLeast = 256;
+// Where no row can hold more keys, each is one chunk and nothing is joined: one launch instead of two. On one row of 333
+// keys 6.2 us, against 5.6 + 4.2 split in two.
+constexpr int kOne = 512;
+// Rows of the join (requests by heads) up to which a workgroup joins one head only, with many threads along the chunks.
+constexpr int kFewRows = 512;
 
+int columns_of(const AttendArgs& a) { return a.kv_heads * ((a.heads / a.kv_heads + kHeads - 1) / kHeads); }
+
+// Four workgroups fit a CU. One request is divided evenly, so that many chunks end together; several leave remainders,
+// which finer chunks spread: 2048 workgroups took 192 us where 1024 took 215 (128 ragged rows, e4m3), and on one row of
+// 131071 keys 98.5 where 1024 took 95.7.
 int target_of(const AttendArgs& a) {
-  int group = a.heads / a.kv_heads, columns = a.kv_heads * ((group + kHeads - 1) / kHeads);
-  int wanted = kWorkgroups / columns;
-  return wanted < 1 ? 1 : wanted;
+  int64_t room = (int64_t)a.width << a.page_log2;
+  if (room <= kOne) return 0;
+  int64_t wanted = (a.requests == 1 ? 1024 : 2048) / columns_of(a), most = (a.requests * room + kLeast - 1) / kLeast;
+  return (int)(wanted < 1 ? 1 : (wanted < most ? wanted : most));
 }
-// no row can have a second chunk
-bool one_chunk(const AttendArgs& a) { return ((int64_t)a.width << a.page_log2) <= kLeast; }
 
 }  // namespace
 
 int64_t decode_workspace(const AttendArgs& a) {
-  return one_chunk(a) ? 0 : ((int64_t)a.requests + target_of(a)) * a.heads * (a.dim + 2);
+  int target = target_of(a);
+  return target ? ((int64_t)a.requests + target) * a.heads * (a.dim + 2) : 0;
 }
 
 bool decode_takes(const AttendArgs& a) { return a.dim == 64 || a.dim == 128; }
@@ -368,22 +406,22 @@ bool decode_takes(const AttendArgs& a) { return a.dim == 64 || a.dim == 128; }
 hipError_t launch_decode(const AttendArgs& a, float* workspace, hipStream_t stream) {
   SplitArgs s;
   s.a = a;
-  s.target = target_of(a), s.least = kLeast;
-  bool single = one_chunk(a);
-  int64_t items = single ? a.requests : (int64_t)a.requests + s.target;
+  int target = target_of(a);
+  s.target = target ? target : 1, s.least = target ? kLeast : kOne;
+  int64_t items = (int64_t)a.requests + target;
   s.part = workspace, s.stats = workspace + items * a.heads * a.dim;
   s.q_wide = (uintptr_t)a.q % 16 == 0 && (a.q_row | a.q_head) % 8 == 0;
-  int group = a.heads / a.kv_heads;
-  dim3 grid((unsigned)items, (unsigned)(a.kv_heads * ((group + kHeads - 1) / kHeads)));
-#define LAUNCH(X, C) \
-  (a.dim == 64 ? launch(split_kernel<X, C, 64>, grid, kWaves * 64, stream, s) : launch(split_kernel<X, C, 128>, grid, kWaves * 64, stream, s))
+  dim3 grid((unsigned)items, (unsigned)columns_of(a));
+#define LAUNCH(X, C) (a.dim == 64 ? launch(split_kernel<X, C, 64>, grid, kWaves * 64, stream, s) : launch(split_kernel<X, C, 128>, grid, kWaves * 64, stream, s))
   hipError_t status = PAGED_DISPATCH(a.type, a.cache, LAUNCH);
 #undef LAUNCH
-  if (status != hipSuccess || single) return status;
-  dim3 rows((unsigned)a.requests, (unsigned)a.heads);
-  if (a.type == Type::kBF16)
-    return a.dim == 64 ? launch(join_kernel<BF16, 64>, rows, kWaves * 64, stream, s) : launch(join_kernel<BF16, 128>, rows, kWaves * 64, stream, s);
-  return a.dim == 64 ? launch(join_kernel<FP16, 64>, rows, kWaves * 64, stream, s) : launch(join_kernel<FP16, 128>, rows, kWaves * 64, stream, s);
+  if (status != hipSuccess || !target) return status;
+  bool few = (int64_t)a.requests * a.heads <= kFewRows;
+  dim3 rows((unsigned)a.requests, (unsigned)(few ? a.heads : (a.heads + 7) / 8));
+#define LAUNCH(X, D) (few ? launch(join_kernel<X, D, 1>, rows, kWaves * 64, stream, s) : launch(join_kernel<X, D, 8>, rows, kWaves * 64, stream, s))
+  if (a.type == Type::kBF16) return a.dim == 64 ? LAUNCH(BF16, 64) : LAUNCH(BF16, 128);
+  return a.dim == 64 ? LAUNCH(FP16, 64) : LAUNCH(FP16, 128);
+#undef LAUNCH
 }
 
 }  // namespace paged

@@ -415,6 +415,30 @@ def test_later_tokens_do_not_reach_earlier_rows(device, dim, bad):
 
 @both
 @pytest.mark.parametrize("dim", [80, 64, 128])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_values_that_are_not_finite_reach_the_rows_that_see_them(device, dim, bad):
+    gen = torch.Generator().manual_seed(8)
+    lens = [1, 40, 700, 33]
+    k_cache, v_cache, tables, scales = make_cache(gen, lens, 1, dim, 16, "bf16", "bf16", device)
+    cache = (k_cache, v_cache, tables, scales)
+    q = torch.randn((4, 2, dim), generator=gen).to(torch.bfloat16).to(device)
+    for cu in (None, [0, 1, 2, 3, 4]):
+        run = lambda: run_decode(q, cache, lens) if cu is None else run_prompt(q, cache, lens, cu)  # noqa: E731
+        clean = run()
+        keep = v_cache.clone()
+        for r, n in enumerate(lens[:3]):
+            v_cache[tables[r][(n - 1) // 16], 0, (n - 1) % 16, 5] = bad
+        got = run()
+        v_cache.copy_(keep)
+        assert torch.equal(got[3], clean[3])
+        assert torch.equal(got[:3, :, 5].float().nan_to_num(3.0, 1.0, -1.0), torch.full((3, 2), bad, device=device).nan_to_num(3.0, 1.0, -1.0))
+        want, off = attention_oracle(q, k_cache, v_cache, tables, lens, [0, 1, 2, 3, 4], dim**-0.5, *scales)
+        rest = [d for d in range(dim) if d != 5]
+        assert ((got.cpu().double() - want).abs() <= off)[..., rest].all()
+
+
+@both
+@pytest.mark.parametrize("dim", [80, 64, 128])
 def test_scores_far_apart(device, dim):
     """Scores of thousands, all equal scores, and a maximum that comes first or last."""
     gen = torch.Generator().manual_seed(6)
