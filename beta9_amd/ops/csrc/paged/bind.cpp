@@ -192,6 +192,7 @@ Tensor attend(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, con
     check_gpu(out, q, "out");
     TORCH_CHECK_TYPE(out.scalar_type() == q.scalar_type(), "out must be ", q.scalar_type(), " like q, is ", out.scalar_type());
     REQUIRE(out.sizes() == q.sizes() && out.is_contiguous(), "out must be contiguous and of q's shape");
+    REQUIRE((uintptr_t)out.data_ptr() % 16 == 0, "out must begin on 16 bytes");
     auto begin = [](const Tensor& t) { return (const char*)t.data_ptr(); };
     int64_t q_span = q.numel() ? ((q.size(0) - 1) * q.stride(0) + (q.size(1) - 1) * q.stride(1) + dim) * 2 : 0;
     REQUIRE(begin(out) + out.numel() * 2 <= begin(q) || begin(q) + q_span <= begin(out) || !out.numel(), "out must not overlap q");
@@ -211,6 +212,10 @@ Tensor attend(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, con
     int64_t floats = paged::decode_workspace(a);
     if (floats) workspace = at::empty({floats}, q.options().dtype(at::kFloat));
     launched(paged::launch_decode(a, floats ? workspace.data_ptr<float>() : nullptr, current_stream()), "decode_attention");
+    return out;
+  }
+  if (cu_new && paged::prompt_takes(a)) {
+    launched(paged::launch_prompt(a, current_stream()), "prompt_attention");
     return out;
   }
   launched(paged::launch_attend_rows(a, current_stream()), cu_new ? "prompt_attention" : "decode_attention");
