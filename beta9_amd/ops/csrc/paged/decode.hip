@@ -29,11 +29,11 @@ template <int N> using Words = uint32_t __attribute__((ext_vector_type(N)));
 
 struct SplitArgs {
   AttendArgs a;
-  float* part;   // [items, heads, dim]: unnormalised sums
-  float* stats;  // [items, heads, 2]: running maximum and sum
-  int target;    // chunks wanted for all requests together; there are at most target + requests
-  int least;     // keys of a chunk at least, a multiple of kWaves * kTile
-  int q_wide;    // q's rows begin on 16 bytes
+  float* part;      // [items, heads, dim]: unnormalised sums
+  float* stats;     // [items, heads, 2]: running maximum and sum
+  int target_log2;  // chunks wanted for all requests together; there are at most as many more as requests
+  int least;        // keys of a chunk at least, a multiple of kWaves * kTile
+  int q_wide;       // q's rows begin on 16 bytes
 };
 
 struct Share {
@@ -46,17 +46,16 @@ struct Share {
 __device__ inline Share share_of(const SplitArgs& s, int item, int request_wanted) {
   const AttendArgs& a = s.a;
   int lane = threadIdx.x & 63;
-  int64_t room = (int64_t)a.width << a.page_log2;
-  auto length = [&](int i) {
-    int l = i < a.requests ? a.kv_lens[i] : 0;
-    return (int)max((int64_t)0, min((int64_t)l, room));
-  };
+  auto length = [&](int i) { return clamp_int(i < a.requests ? a.kv_lens[i] : 0, 0, a.width << a.page_log2); };
   int mine = length(lane);  // the first 64 requests' lengths stay here for both passes
-  int64_t total = mine;
-  for (int i = lane + 64; i < a.requests; i += 64) total += length(i);
-#pragma unroll
-  for (int m = 32; m; m >>= 1) total += __shfl_xor((long long)total, m);
-  int64_t even = (total + s.target - 1) / s.target;
+  // lengths are at most 2^30, requests 4096: the sums of their lower 16 bits and of the rest fit 32
+  int low = mine & 0xffff, high = mine >> 16;
+  for (int i = lane + 64; i < a.requests; i += 64) {
+    int l = length(i);
+    low += l & 0xffff, high += l >> 16;
+  }
+  int64_t total = ((int64_t)whole_sum(high) << 16) + whole_sum(low);
+  int64_t even = (total + (1 << s.target_log2) - 1) >> s.target_log2;
   constexpr int kStep = kWaves * kTile;
   uint32_t chunk = (uint32_t)min((int64_t)1 << 31, max((int64_t)s.least, (even + kStep - 1) / kStep * kStep));
   int before = 0;
@@ -64,20 +63,14 @@ __device__ inline Share share_of(const SplitArgs& s, int item, int request_wante
     int i = first + lane, l = first ? length(i) : mine;
     // a request without keys has one chunk all the same: its zeros
     int n = i < a.requests ? max(1, (int)(((uint32_t)l + chunk - 1u) / chunk)) : 0;
-    int up = n;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      int y = __shfl_up(up, d);
-      if (lane >= d) up += y;
-    }
+    int up = running_sum(n);
     bool here = request_wanted >= 0 ? i == request_wanted : before + up > item;
     uint64_t found = __ballot(here && i < a.requests);
     if (found) {
-      int at = __builtin_ctzll(found);
-      int start = before + __shfl(up, at) - __shfl(n, at);
-      return {first + at, __shfl(l, at), chunk, request_wanted >= 0 ? start : item - start, __shfl(n, at)};
+      int at = __builtin_ctzll(found), count = lane_value(n, at), start = before + lane_value(up, at) - count;
+      return {first + at, lane_value(l, at), chunk, request_wanted >= 0 ? start : item - start, count};
     }
-    before += __shfl(up, 63);
+    before += lane_value(up, 63);
   }
   return {-1, 0, 0, 0, 0};
 }
@@ -387,18 +380,24 @@ int columns_of(const AttendArgs& a) { return a.kv_heads * ((a.heads / a.kv_heads
 // Four workgroups fit a CU. One request is divided evenly, so that many chunks end together; several leave remainders,
 // which finer chunks spread: 2048 workgroups took 192 us where 1024 took 215 (128 ragged rows, e4m3), and on one row of
 // 131071 keys 98.5 where 1024 took 95.7.
-int target_of(const AttendArgs& a) {
+// Powers of two, for the division in the kernel. -1: all rows are one chunk.
+int target_log2_of(const AttendArgs& a) {
   int64_t room = (int64_t)a.width << a.page_log2;
-  if (room <= kOne) return 0;
+  if (room <= kOne) return -1;
   int64_t wanted = (a.requests == 1 ? 1024 : 2048) / columns_of(a), most = (a.requests * room + kLeast - 1) / kLeast;
-  return (int)(wanted < 1 ? 1 : (wanted < most ? wanted : most));
+  int log2 = 0;
+  while ((2LL << log2) <= wanted && (1LL << log2) < most) log2++;
+  return log2;
+}
+int64_t items_of(const AttendArgs& a) {
+  int log2 = target_log2_of(a);
+  return (int64_t)a.requests + (log2 < 0 ? 0 : 1LL << log2);
 }
 
 }  // namespace
 
 int64_t decode_workspace(const AttendArgs& a) {
-  int target = target_of(a);
-  return target ? ((int64_t)a.requests + target) * a.heads * (a.dim + 2) : 0;
+  return target_log2_of(a) < 0 ? 0 : items_of(a) * a.heads * (a.dim + 2);
 }
 
 bool decode_takes(const AttendArgs& a) { return a.dim == 64 || a.dim == 128; }
@@ -406,16 +405,18 @@ bool decode_takes(const AttendArgs& a) { return a.dim == 64 || a.dim == 128; }
 hipError_t launch_decode(const AttendArgs& a, float* workspace, hipStream_t stream) {
   SplitArgs s;
   s.a = a;
-  int target = target_of(a);
-  s.target = target ? target : 1, s.least = target ? kLeast : kOne;
-  int64_t items = (int64_t)a.requests + target;
+  int log2 = target_log2_of(a);
+  bool split = log2 >= 0;
+  // not split: chunks of kOne, whatever the sum of the lengths is
+  s.target_log2 = split ? log2 : 30, s.least = split ? kLeast : kOne;
+  int64_t items = items_of(a);
   s.part = workspace, s.stats = workspace + items * a.heads * a.dim;
   s.q_wide = (uintptr_t)a.q % 16 == 0 && (a.q_row | a.q_head) % 8 == 0;
   dim3 grid((unsigned)items, (unsigned)columns_of(a));
 #define LAUNCH(X, C) (a.dim == 64 ? launch(split_kernel<X, C, 64>, grid, kWaves * 64, stream, s) : launch(split_kernel<X, C, 128>, grid, kWaves * 64, stream, s))
   hipError_t status = PAGED_DISPATCH(a.type, a.cache, LAUNCH);
 #undef LAUNCH
-  if (status != hipSuccess || !target) return status;
+  if (status != hipSuccess || !split) return status;
   bool few = (int64_t)a.requests * a.heads <= kFewRows;
   dim3 rows((unsigned)a.requests, (unsigned)(few ? a.heads : (a.heads + 7) / 8));
 #define LAUNCH(X, D) (few ? launch(join_kernel<X, D, 1>, rows, kWaves * 64, stream, s) : launch(join_kernel<X, D, 8>, rows, kWaves * 64, stream, s))

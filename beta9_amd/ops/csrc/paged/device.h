@@ -61,6 +61,33 @@ __device__ inline float wave_sum(float x) {
   return x;
 }
 
+// Inclusive sums, the sum and the maximum over the lanes of whole numbers, by moves within the registers: about 50 cycles,
+// where exchanges through LDS take 130 for each of the six steps.
+template <int kControl, int kRows> __device__ inline int moved(int x, int otherwise) {
+  return __builtin_amdgcn_update_dpp(otherwise, x, kControl, kRows, 0xf, false);
+}
+__device__ inline int running_sum(int x) {
+  x += moved<0x111, 0xf>(x, 0);  // row_shr 1, 2, 4, 8: within 16 lanes
+  x += moved<0x112, 0xf>(x, 0);
+  x += moved<0x114, 0xf>(x, 0);
+  x += moved<0x118, 0xf>(x, 0);
+  x += moved<0x142, 0xa>(x, 0);  // the last lane of rows 0 and 2 to rows 1 and 3
+  x += moved<0x143, 0xc>(x, 0);  // the last lane of the first half to the second
+  return x;
+}
+__device__ inline int lane_value(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
+__device__ inline int whole_sum(int x) { return lane_value(running_sum(x), 63); }
+// of values that are not negative
+__device__ inline int whole_max(int x) {
+  x = max(x, moved<0x111, 0xf>(x, 0));
+  x = max(x, moved<0x112, 0xf>(x, 0));
+  x = max(x, moved<0x114, 0xf>(x, 0));
+  x = max(x, moved<0x118, 0xf>(x, 0));
+  x = max(x, moved<0x142, 0xa>(x, 0));
+  x = max(x, moved<0x143, 0xc>(x, 0));
+  return lane_value(x, 63);
+}
+
 // Which request the packed row belongs to: the last i with cu[i] <= row, cu[requests] > row being known.
 __device__ inline int request_of(const int* cu, int requests, int row) {
   int low = 0, high = requests;

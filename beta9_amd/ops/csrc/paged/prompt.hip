@@ -12,6 +12,7 @@
 // So the probabilities never leave their registers and a row's maximum and sum are one lane's, but for one exchange between
 // the two halves. Rows of LDS are 128 or 256 bytes, and the 16-byte chunks of a row are exchanged by its number so that the
 // reads of eight rows' same chunk (K) and of four rows' same two chunks (V) meet no bank twice.
+// LDS is one array, this kernel's own: with another beside it the compiler waits for the loads into LDS before it reads.
 //
 // What bounds it is the matrix instructions, the exponentials (as many cycles, nearly) and LDS (128 bytes a cycle for one
 // operand of each instruction) together.
@@ -31,6 +32,7 @@ struct PromptArgs {
   AttendArgs a;
   int q_wide;    // q's rows begin on 16 bytes
   int negative;  // the scale is below zero: q's sign is turned instead
+  int group, group_log2, kv_heads_log2;  // logarithms: -1 where there is none
 };
 
 template <class X> struct Product;
@@ -62,74 +64,154 @@ __device__ inline u32x2 read_turned(const char* p) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p)));
 }
 
-struct Where {
-  int request, tile, row0, rows;  // the request's first packed row and its new tokens
+// 16 bytes a lane from `from` + `at` bytes to LDS at `to` + 16 * lane. By hand, since the compiler takes a transposing read
+// of LDS for one that may meet any load into LDS on its way, and would wait for the next tile there. It writes no register,
+// and what it brings is read after a wait for it and a barrier.
+__device__ inline void load_into_lds(const char* from, uint32_t at, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(at), "s"(from), "s"(to) : "memory", "m0");
+}
+
+template <int N> struct Constant {
+  constexpr operator int() const { return N; }
 };
 
-// Which rows the item stands for; tiles of a request last to first, since the last see the most keys. request -1: none.
-__device__ inline Where where_of(const AttendArgs& a, int item) {
-  int lane = threadIdx.x & 63, group = a.heads / a.kv_heads, before = 0;
+struct Where {
+  int request, tile, row0, rows, keys;  // the request's first packed row, its new tokens and all of them
+};
+
+// Which rows the item stands for. The tiles that see the most keys come first, so that the last workgroups to start are
+// short ones: up to 64 requests, all tiles are put in order of their last position, in 64 steps (a lane a step counts the
+// tiles in it); among more, the requests follow each other, each from its last tile to its first. On 13 ragged prompts
+// (16 heads of 64, up to 1500 new tokens) 75.8 us, in the requests' order 77.9.
+__device__ inline Where where_of(const AttendArgs& a, int group, int item) {
+  int lane = threadIdx.x & 63, before = 0;
   for (int first = 0; first < a.requests; first += 64) {
-    int i = first + lane, row0 = 0, n = 0;
+    int i = first + lane, row0 = 0, n = 0, keys = 0;
     if (i < a.requests) {
       row0 = clamp_int(a.cu_new[i], 0, a.rows);
       n = clamp_int(a.cu_new[i + 1], row0, a.rows) - row0;
+      keys = clamp_int(a.kv_lens[i], 0, a.width << a.page_log2);
     }
-    int tiles = (int)(((int64_t)n * group + kRows - 1) / kRows), up = tiles;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      int y = __shfl_up(up, d);
-      if (lane >= d) up += y;
+    int tiles = (int)(((int64_t)n * group + kRows - 1) / kRows), from = 0, mine = tiles;
+    if (a.requests > 1 && a.requests <= 64) {
+      // in tiles' places: the request's begin behind what it held before
+      int start = (int)(min((int64_t)max(keys - n, 0) * group, (int64_t)1 << 30) / kRows), end = start + tiles;
+      int width = (whole_max(end) + 63) / 64, low = (63 - lane) * width, count = 0;
+      for (int r = 0; r < a.requests; r++)
+        count += clamp_int(lane_value(end, r) - low, 0, width) - clamp_int(lane_value(start, r) - low, 0, width);
+      int up = running_sum(count);
+      uint64_t found = __ballot(up > item);
+      if (!found) break;
+      int at = __builtin_ctzll(found);
+      item -= lane_value(up, at) - lane_value(count, at);
+      low = (63 - at) * width;
+      from = clamp_int(low - start, 0, tiles);
+      mine = clamp_int(low + width - start, 0, tiles) - from;
     }
+    int up = running_sum(mine);
     uint64_t found = __ballot(before + up > item);
     if (found) {
       int at = __builtin_ctzll(found);
-      return {first + at, before + __shfl(up, at) - 1 - item, __shfl(row0, at), __shfl(n, at)};
+      return {first + at, lane_value(from, at) + before + lane_value(up, at) - 1 - item, lane_value(row0, at), lane_value(n, at), lane_value(keys, at)};
     }
-    before += __shfl(up, 63);
+    before += lane_value(up, 63);
   }
-  return {-1, 0, 0, 0};
+  return {-1, 0, 0, 0, 0};
 }
 
 template <class X, class C, int D>
-__global__ __launch_bounds__(kWaves * 64, 2) void prompt_kernel(PromptArgs s) {
+__global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : 2) void prompt_kernel(PromptArgs s) {
   typedef typename Vec<X>::x8 Half8;
   typedef typename X::T Out;
   constexpr bool kNarrow = sizeof(typename C::T) == 1;
   constexpr float kBias = __is_same(X, FP16) ? 8.f : 0.f;   // see the kernel of one token
   constexpr float kSlack = __is_same(X, FP16) ? 6.f : 8.f;  // how far a score may pass the maximum before the sums are rescaled
+  constexpr bool kAhead = D == 128;
   constexpr int kSteps = D / 16, kDims = D / 32;
   constexpr int kRowBytes = D * 2, kChunks = D / 8, kTileBytes = kKeys * kRowBytes;
-  __shared__ __attribute__((aligned(16))) char lds[2 * 2 * kTileBytes];  // [buffer][K, V][key][dim]
+  __shared__ __attribute__((aligned(16))) char lds[2 * 2 * kTileBytes];  // [K, V][buffer][key][dim]
   const AttendArgs& a = s.a;
   int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5, n = lane & 31;
-  int item = blockIdx.x / a.kv_heads, kv_head = blockIdx.x - item * a.kv_heads;
+  int item = s.kv_heads_log2 >= 0 ? blockIdx.x >> s.kv_heads_log2 : blockIdx.x / a.kv_heads, kv_head = blockIdx.x - item * a.kv_heads;
 
-  if (a.clear_rest) {
+  auto clear_rest = [&]() {
+    if (!a.clear_rest) return;
     int rest = clamp_int(a.cu_new[a.requests], 0, a.rows), front = clamp_int(a.cu_new[0], 0, a.rows);
     for (int64_t r = blockIdx.x; r < front + (int64_t)a.rows - rest; r += gridDim.x) {
       Out* out = (Out*)a.out + (r < front ? r : r - front + rest) * a.out_row;
       for (int i = tid; i < a.heads * D; i += kWaves * 64) out[(i / D) * a.out_head + i % D] = (Out)0.f;
     }
+  };
+  Where w = where_of(a, s.group, item);
+  if (w.request < 0) {
+    clear_rest();
+    return;
   }
-  Where w = where_of(a, item);
-  if (w.request < 0) return;
-  int group = a.heads / a.kv_heads;
-  int packed = __builtin_amdgcn_readfirstlane(w.rows) * group;  // fits: rows by heads do
-  int64_t room = (int64_t)a.width << a.page_log2;
-  int length = __builtin_amdgcn_readfirstlane((int)max((int64_t)0, min((int64_t)a.kv_lens[w.request], room)));
+  int group = s.group;
+  auto by_group = [&](int x) { return s.group_log2 >= 0 ? x >> s.group_log2 : x / group; };
+  int packed = w.rows * group;  // fits: rows by heads do
+  int length = w.keys;
   int ahead = length - w.rows;  // a token's position less its number among the new ones
-  int row_first = __builtin_amdgcn_readfirstlane(w.tile) * kRows, wave_first = row_first + wave * 32;
+  int row_first = w.tile * kRows, wave_first = row_first + wave * 32;
   int row = wave_first + n;
   bool real = row < packed;
-  int token = min(row, packed - 1) / group, head = kv_head * group + min(row, packed - 1) - token * group;
+  int token = by_group(min(row, packed - 1)), head = kv_head * group + min(row, packed - 1) - token * group;
   int position = ahead + token;
-  int low = ahead + min(wave_first, packed - 1) / group, high = ahead + min(wave_first + 31, packed - 1) / group;
-  int last = ahead + min(row_first + kRows - 1, packed - 1) / group;  // the workgroup's last position
+  int low = ahead + by_group(min(wave_first, packed - 1)), high = ahead + by_group(min(wave_first + 31, packed - 1));
+  int last = ahead + by_group(min(row_first + kRows - 1, packed - 1));  // the workgroup's last position
   int tiles = last < 0 ? 0 : min(last, length - 1) / kKeys + 1;
 
+  const int* table = a.tables + w.request * a.table_stride;
+  const char* caches[2] = {(const char*)a.k_cache, (const char*)a.v_cache};
+  int in_page = (1 << a.page_log2) - 1;
+  // the entry of the lane's key of a tile, and of the key's row of the cache
+  auto entry_of = [&](int tile) { return table[min((tile * kKeys + lane) >> a.page_log2, a.width - 1)]; };
+  auto cache_row = [&](int entry, int key) {
+    uint32_t page = (unsigned)entry < (unsigned)a.pages ? entry : 0;
+    return ((page * a.kv_heads + kv_head) << a.page_log2) + (key & in_page);  // memory holds fewer than 2^32 rows
+  };
+  // which chunk of a key's row lies at place 0: differs for the 16 rows that a read of K covers, and by more than the pairs
+  // that a read of V covers for four neighbouring rows
+  auto swizzle = [](int key) { return D == 128 ? (key & 3) << 2 | (key >> 2 & 3) : (key & 2) << 1 | (key >> 2 & 3); };
+
+  // 16-bit: straight into LDS, 1 KB an instruction, which lie in one page; the lanes fetch what belongs at their place
+  constexpr int kPieceKeys = 1024 / kRowBytes, kPieces = kTileBytes / 1024 / kWaves;
+  uint32_t lds_base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds) + wave * 1024;
+  int piece_key = lane / kChunks;
+  uint32_t piece_at = piece_key * kRowBytes + (((lane % kChunks) ^ swizzle(wave * kPieceKeys + piece_key)) * 16);
+  auto stage = [&](int side, int tile, int buffer, int entry) {
+    uint32_t row = cache_row(entry, lane);  // the low bits of a key are its place in the tile: a tile begins on 64
+    if (a.page_log2 > 6) row += (tile * kKeys) & in_page & ~(kKeys - 1);
+#pragma unroll
+    for (int i = 0; i < kPieces; i++)
+      load_into_lds(caches[side] + (uint64_t)(uint32_t)__builtin_amdgcn_readlane(row, (wave + kWaves * i) * kPieceKeys) * kRowBytes, piece_at,
+                    lds_base + (2 * side + buffer) * kTileBytes + kWaves * i * 1024);
+  };
+  // 8-bit: through registers, widened on the way to LDS
+  constexpr int kUnits = kKeys * D / 16 / (kWaves * 64);  // 16 dims each
+  u32x4 narrow[kNarrow ? kUnits : 1];
+  auto fetch = [&](int side, int tile, int entry) {
+#pragma unroll
+    for (int i = 0; i < kUnits; i++) {
+      int unit = tid + i * kWaves * 64, key = unit / (D / 16);
+      uint64_t row = cache_row(__shfl(entry, key), tile * kKeys + key);
+      narrow[i] = *reinterpret_cast<const u32x4*>(caches[side] + row * D + (unit % (D / 16)) * 16);
+    }
+  };
+  auto put = [&](int side, int buffer) {
+#pragma unroll
+    for (int i = 0; i < kUnits; i++) {
+      int unit = tid + i * kWaves * 64, key = unit / (D / 16), chunk = (unit % (D / 16)) * 2;
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        u32x2 x = {narrow[i][2 * j], narrow[i][2 * j + 1]};
+        *reinterpret_cast<u32x4*>(lds + (2 * side + buffer) * kTileBytes + key * kRowBytes + ((chunk + j) ^ swizzle(key)) * 16) = widen8<X>(x);
+      }
+    }
+  };
+
   Half8 q[kSteps];
-  {
+  auto load_q = [&]() {
     const Out* p = (const Out*)a.q + (w.row0 + token) * a.q_row + head * a.q_head + half * 8;
 #pragma unroll
     for (int i = 0; i < kSteps; i++) {
@@ -145,185 +227,262 @@ __global__ __launch_bounds__(kWaves * 64, 2) void prompt_kernel(PromptArgs s) {
       if (s.negative) x = -x;
       q[i] = x;
     }
-  }
-
-  const int* table = a.tables + w.request * a.table_stride;
-  const typename C::T* caches[2] = {(const typename C::T*)a.k_cache, (const typename C::T*)a.v_cache};
-  int in_page = (1 << a.page_log2) - 1;
-  // the entry of the lane's key of a tile
-  auto entry_of = [&](int tile) { return table[min((tile * kKeys + lane) >> a.page_log2, a.width - 1)]; };
-  auto swizzle = [](int key) { return D == 128 ? (key & 7) << 1 : ((key >> 1) & 3) << 1; };
-
-  // 16-bit: straight into LDS, 1 KB an instruction, which lie in one page; the lanes fetch what belongs at their place
-  constexpr int kPieceKeys = 1024 / kRowBytes, kPieces = kTileBytes / 1024 / kWaves;
-  int piece_key = lane / kChunks;
-  int piece_at = piece_key * D + (((lane % kChunks) ^ swizzle(wave * kPieceKeys + piece_key)) * 8);
-  auto stage = [&](int tile, int buffer, int entry) {
-#pragma unroll
-    for (int i = 0; i < kPieces; i++) {
-      int piece = wave + kWaves * i, key = tile * kKeys + piece * kPieceKeys;
-      int page = __builtin_amdgcn_readlane(entry, piece * kPieceKeys);
-      page = (unsigned)page < (unsigned)a.pages ? page : 0;
-      int64_t at = ((((int64_t)page * a.kv_heads + kv_head) << a.page_log2) + (key & in_page)) * D;
-#pragma unroll
-      for (int side = 0; side < 2; side++)
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)(caches[side] + at + piece_at),
-                                         (__attribute__((address_space(3))) uint32_t*)(lds + (buffer * 2 + side) * kTileBytes + piece * 1024),
-                                         16, 0, 0);
-    }
   };
-  // 8-bit: through registers, widened on the way to LDS
-  constexpr int kUnits = kKeys * D / 16 / (kWaves * 64);  // 16 dims each
-  u32x4 narrow[2][kNarrow ? kUnits : 1];
-  auto fetch = [&](int tile, int entry) {
-#pragma unroll
-    for (int i = 0; i < kUnits; i++) {
-      int unit = tid + i * kWaves * 64, key = unit / (D / 16), page = __shfl(entry, key);
-      page = (unsigned)page < (unsigned)a.pages ? page : 0;
-      int64_t at = ((((int64_t)page * a.kv_heads + kv_head) << a.page_log2) + ((tile * kKeys + key) & in_page)) * D + (unit % (D / 16)) * 16;
-#pragma unroll
-      for (int side = 0; side < 2; side++) narrow[side][i] = *reinterpret_cast<const u32x4*>(caches[side] + at);
-    }
-  };
-  auto put = [&](int buffer) {
-#pragma unroll
-    for (int i = 0; i < kUnits; i++) {
-      int unit = tid + i * kWaves * 64, key = unit / (D / 16), chunk = (unit % (D / 16)) * 2;
-#pragma unroll
-      for (int side = 0; side < 2; side++)
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-          u32x2 x = {narrow[side][i][2 * j], narrow[side][i][2 * j + 1]};
-          *reinterpret_cast<u32x4*>(lds + (buffer * 2 + side) * kTileBytes + key * kRowBytes + ((chunk + j) ^ swizzle(key)) * 16) = widen8<X>(x);
-        }
-    }
-  };
-
   f32x16 acc[kDims];
   float m, l;
   int k_at = n * kRowBytes + ((half ^ swizzle(n)) << 4);
   int quarter = lane >> 4, in_quarter = lane & 15, v_key = 4 * half + (in_quarter >> 2);
-  int v_at = v_key * kRowBytes + ((((quarter & 1) * 2 + ((in_quarter & 3) >> 1)) ^ swizzle(v_key)) << 4) + (in_quarter & 1) * 8;
+  int v_chunk = (quarter & 1) * 2 + ((in_quarter & 3) >> 1), v_rest = (in_quarter & 1) * 8;
+  int v_at = v_key * kRowBytes + ((v_chunk ^ swizzle(v_key)) << 4) + v_rest;
+  int v_at8 = (v_key + 8) * kRowBytes + ((v_chunk ^ swizzle(v_key + 8)) << 4) + v_rest;
 
-  // One pass over the keys. A later token's value that is not finite would reach the rows that do not see it through
-  // 0 * inf; `careful` takes the keys of a tile one by one where a row may not see them all.
+  // The scores of a tile that is in LDS.
+  auto scores = [&](int buffer, f32x16 (&x)[2]) {
+    const char* k_lds = lds + buffer * kTileBytes;
+#pragma unroll
+    for (int h = 0; h < 2; h++) x[h] = f32x16{};
+#pragma unroll
+    for (int i = 0; i < kSteps; i++)
+#pragma unroll
+      for (int h = 0; h < 2; h++)
+        x[h] = Product<X>::of(*reinterpret_cast<const Half8*>(k_lds + h * 32 * kRowBytes + (k_at ^ (i * 32))), q[i], x[h]);
+  };
+  // Leaves out what a row does not see, and raises the running maximum if it must.
+  auto mask = [&](f32x16 (&x)[2], int key0, uint64_t present) {
+    bool whole = key0 + kKeys - 1 <= low && present == ~0ull;
+    if (!whole) {
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        // bit 8 (r / 4) + r % 4 of a half's 32: whether the row sees the key; keys past the length lie past the position
+        int count = position - key0 - 32 * h + 1;
+        uint32_t seen = count <= 0 ? 0u : (count >= 32 ? ~0u : (1u << count) - 1u);
+        seen = (seen & (uint32_t)(present >> (32 * h))) >> (4 * half);
+#pragma unroll
+        for (int r = 0; r < 16; r++) x[h][r] = seen >> (8 * (r >> 2) + (r & 3)) & 1 ? x[h][r] : kMinusInf;
+      }
+    }
+    return whole;
+  };
+  auto highest = [&](const f32x16 (&x)[2]) {
+    float top = kMinusInf;
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) top = fmaxf(top, x[h][r]);
+    return top;
+  };
+  auto raise = [&](float top) {
+    if (__any(top * a.score_scale > m + kSlack)) {
+      top = fmaxf(top, __shfl_xor(top, 32)) * a.score_scale;
+      top = fmaxf(m, top);
+      float alpha = top == kMinusInf ? 1.f : __builtin_amdgcn_exp2f(m - top);
+      m = top;
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < kDims; d++) acc[d] *= alpha;
+    }
+  };
+  auto weigh = [&](const f32x16 (&x)[2], Half8 (&p)[4]) {
+    float from = (m == kMinusInf ? 0.f : m) - kBias;
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        float y = __builtin_amdgcn_exp2f(__builtin_fmaf(x[h][r], a.score_scale, -from));
+        l += y;
+        p[2 * h + (r >> 3)][r & 7] = (typename X::T)y;  // rounded for the matrix product; the sum l is not
+      }
+  };
+  auto v_operand = [&](int buffer, int step, int d) {
+    const char* v = lds + (2 + buffer) * kTileBytes + step * 16 * kRowBytes;
+    u32x2 lo = read_turned(v + (v_at ^ (d * 64))), hi = read_turned(v + (v_at8 ^ (d * 64)));
+    return u32x4{lo[0], lo[1], hi[0], hi[1]};
+  };
+  auto values = [&](int buffer, const Half8 (&p)[4]) {
+#pragma unroll
+    for (int step = 0; step < 4; step++)
+#pragma unroll
+      for (int d = 0; d < kDims; d++) acc[d] = Product<X>::of(__builtin_bit_cast(Half8, v_operand(buffer, step, d)), p[step], acc[d]);
+  };
+  // The same, key by key, for the rows that see the key.
+  auto values_seen = [&](int buffer, const Half8 (&p)[4], int key0, uint64_t present) {
+#pragma unroll
+    for (int step = 0; step < 4; step++)
+#pragma unroll 1
+      for (int key = 0; key < 16; key++) {
+        // operand element j of half hh stands for key 8 (j / 4) + 4 hh + j % 4
+        int hh = key >> 2 & 1, j = (key >> 3) * 4 + (key & 3);
+        bool sees = key0 + 16 * step + key <= position && (present >> (16 * step + key) & 1);
+        u32x4 only;
+#pragma unroll
+        for (int i = 0; i < 4; i++) only[i] = hh == half && (j >> 1) == i ? (j & 1 ? 0xffff0000u : 0xffffu) : 0u;
+        u32x4 py = __builtin_bit_cast(u32x4, p[step]) & only;
+#pragma unroll
+        for (int d = 0; d < kDims; d++) {
+          f32x16 y = Product<X>::of(__builtin_bit_cast(Half8, v_operand(buffer, step, d) & only), __builtin_bit_cast(Half8, py), acc[d]);
+#pragma unroll
+          for (int r = 0; r < 16; r++) acc[d][r] = sees ? y[r] : acc[d][r];
+        }
+      }
+  };
+  auto present_of = [&](int entry) { return __ballot((unsigned)entry < (unsigned)a.pages); };
+
+  // One pass over the keys. A tile's scores are made in the step before its own, so that the matrix instructions of the
+  // next tile's scores and the exponentials of this one's fill each other's gaps within a wave; K is therefore a tile
+  // ahead of V. A later token's value that is not finite would reach the rows that do not see it through 0 * inf;
+  // `careful` takes the keys of a tile one by one where a row may not see them all.
   auto pass = [&](auto careful) {
 #pragma unroll
     for (int d = 0; d < kDims; d++) acc[d] = f32x16{};
     m = kMinusInf, l = 0.f;
     if (!tiles) return;
-    int entry = entry_of(0), entry_next = entry_of(1);
-    if constexpr (kNarrow) {
-      fetch(0, entry);
-      put(0);
-    } else {
-      stage(0, 0, entry);
-    }
-    for (int tile = 0; tile < tiles; tile++) {
-      int buffer = tile & 1;
-      uint64_t present = __ballot((unsigned)entry < (unsigned)a.pages);
-      if constexpr (!kNarrow) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();  // this tile is in LDS, and nobody reads the other buffer any more
-      if (tile + 1 < tiles) {
-        if constexpr (kNarrow)
-          fetch(tile + 1, entry_next);
-        else
-          stage(tile + 1, buffer ^ 1, entry_next);
+    int mine = high < 0 ? 0 : min(tiles, high / kKeys + 1);  // the wave's own tiles
+    if constexpr (!kAhead) {
+      int entry0 = entry_of(0), entry1 = entry_of(1);
+      if constexpr (kNarrow) {
+        fetch(0, 0, entry0), put(0, 0);
+        fetch(1, 0, entry0), put(1, 0);
+      } else {
+        stage(0, 0, 0, entry0);
+        stage(1, 0, 0, entry0);
       }
-      entry = entry_next;
-      entry_next = entry_of(tile + 2);
-      int key0 = tile * kKeys;
-      if (key0 <= high) {
-        const char* k_lds = lds + buffer * 2 * kTileBytes;
-        const char* v_lds = k_lds + kTileBytes;
-        f32x16 x[2] = {};
-#pragma unroll
-        for (int i = 0; i < kSteps; i++)
-#pragma unroll
-          for (int h = 0; h < 2; h++)
-            x[h] = Product<X>::of(*reinterpret_cast<const Half8*>(k_lds + h * 32 * kRowBytes + (k_at ^ (i * 32))), q[i], x[h]);
-        bool whole = key0 + kKeys - 1 <= low && present == ~0ull;
-        // bit 8 (r / 4) + r % 4 of a half's 32: whether the row sees the key; keys past the length lie past the position
-        uint32_t seen[2];
-        if (!whole) {
-#pragma unroll
-          for (int h = 0; h < 2; h++) {
-            int count = position - key0 - 32 * h + 1;
-            uint32_t mask = count <= 0 ? 0u : (count >= 32 ? ~0u : (1u << count) - 1u);
-            seen[h] = (mask & (uint32_t)(present >> (32 * h))) >> (4 * half);
-#pragma unroll
-            for (int r = 0; r < 16; r++) x[h][r] = seen[h] >> (8 * (r >> 2) + (r & 3)) & 1 ? x[h][r] : kMinusInf;
-          }
-        }
-        float top = kMinusInf;
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-          for (int r = 0; r < 16; r++) top = fmaxf(top, x[h][r]);
-        if (__any(top * a.score_scale > m + kSlack)) {
-          top = fmaxf(top, __shfl_xor(top, 32)) * a.score_scale;
-          top = fmaxf(m, top);
-          float alpha = top == kMinusInf ? 1.f : __builtin_amdgcn_exp2f(m - top);
-          m = top;
-          l *= alpha;
-#pragma unroll
-          for (int d = 0; d < kDims; d++) acc[d] *= alpha;
-        }
-        float from = (m == kMinusInf ? 0.f : m) - kBias;
-        Half8 p[4];
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-          for (int r = 0; r < 16; r++) {
-            float y = __builtin_amdgcn_exp2f(__builtin_fmaf(x[h][r], a.score_scale, -from));
-            l += y;
-            p[2 * h + (r >> 3)][r & 7] = (typename X::T)y;  // rounded for the matrix product; the sum l is not
-          }
-        auto v_operand = [&](int step, int d) {
-          const char* v = v_lds + step * 16 * kRowBytes + (v_at ^ (d * 64));
-          u32x2 lo = read_turned(v), hi = read_turned(v + 8 * kRowBytes);
-          return u32x4{lo[0], lo[1], hi[0], hi[1]};
-        };
-        if (careful && !whole) {
-#pragma unroll
-          for (int step = 0; step < 4; step++)
-#pragma unroll 1
-            for (int key = 0; key < 16; key++) {
-              // operand element j of half hh stands for key 8 (j / 4) + 4 hh + j % 4
-              int hh = key >> 2 & 1, j = (key >> 3) * 4 + (key & 3);
-              bool sees = key0 + 16 * step + key <= position && (present >> (16 * step + key) & 1);
-              u32x4 only;
-#pragma unroll
-              for (int i = 0; i < 4; i++) only[i] = hh == half && (j >> 1) == i ? (j & 1 ? 0xffff0000u : 0xffffu) : 0u;
-              u32x4 py = __builtin_bit_cast(u32x4, p[step]) & only;
-#pragma unroll
-              for (int d = 0; d < kDims; d++) {
-                f32x16 y = Product<X>::of(__builtin_bit_cast(Half8, v_operand(step, d) & only), __builtin_bit_cast(Half8, py), acc[d]);
-#pragma unroll
-                for (int r = 0; r < 16; r++) acc[d][r] = sees ? y[r] : acc[d][r];
-              }
-            }
+      if (!careful) load_q();
+      auto step = [&](auto which, int tile) {
+        constexpr int buffer = which;
+        if constexpr (!kNarrow) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        uint64_t present = present_of(entry0);
+        int entry2 = entry_of(tile + 2);
+        if constexpr (kNarrow) {
+          fetch(0, tile + 1, entry1);
         } else {
-#pragma unroll
-          for (int step = 0; step < 4; step++)
-#pragma unroll
-            for (int d = 0; d < kDims; d++) acc[d] = Product<X>::of(__builtin_bit_cast(Half8, v_operand(step, d)), p[step], acc[d]);
+          stage(0, tile + 1, buffer ^ 1, entry1);
+          stage(1, tile + 1, buffer ^ 1, entry1);
         }
+        f32x16 x[2];
+        bool whole = true;
+        if (tile < mine) {
+          scores(buffer, x);
+          whole = mask(x, tile * kKeys, present);
+          raise(highest(x));
+        }
+        if constexpr (kNarrow) {
+          put(0, buffer ^ 1);
+          fetch(1, tile + 1, entry1);
+        }
+        if (tile < mine) {
+          Half8 p[4];
+          weigh(x, p);
+          if (careful && !whole)
+            values_seen(buffer, p, tile * kKeys, present);
+          else
+            values(buffer, p);
+        }
+        if constexpr (kNarrow) put(1, buffer ^ 1);
+        entry0 = entry1, entry1 = entry2;
+      };
+      for (int tile = 0; tile < tiles; tile += 2) {
+        step(Constant<0>{}, tile);
+        if (tile + 1 < tiles) step(Constant<1>{}, tile + 1);
       }
-      if constexpr (kNarrow)
-        if (tile + 1 < tiles) put(buffer ^ 1);
+      __syncthreads();
+      return;
+    } else {
+    int entry0 = entry_of(0), entry1 = entry_of(1), entry2 = entry_of(2);  // of this tile and the next two
+    if constexpr (kNarrow) {
+      fetch(0, 0, entry0), put(0, 0);
+      fetch(1, 0, entry0), put(1, 0);
+      fetch(0, 1, entry1), put(0, 1);
+    } else {
+      stage(0, 0, 0, entry0);
+      stage(1, 0, 0, entry0);
+      stage(0, 1, 1, entry1);
+    }
+    if (!careful) load_q();
+    if constexpr (!kNarrow) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    f32x16 x[2];
+    scores(0, x);
+    uint64_t present = present_of(entry0);
+    bool whole = mask(x, 0, present);
+    raise(highest(x));
+    // one step: x holds the tile's scores, y takes the next's
+    auto step = [&](auto which, int tile, f32x16 (&x)[2], f32x16 (&y)[2]) {
+      constexpr int buffer = which;
+      constexpr bool careful_now = careful;
+      if constexpr (!kNarrow) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();  // K of the next tile and V of this one are in LDS, and nobody reads the other buffers any more
+      // the last steps load tiles that nobody uses, of the table's last entry
+      int entry3 = entry_of(tile + 3);
+      if constexpr (kNarrow) {
+        fetch(0, tile + 2, entry2);
+      } else {
+        stage(0, tile + 2, buffer, entry2);
+        stage(1, tile + 1, buffer ^ 1, entry1);
+      }
+      if (tile < mine) {
+        Half8 p[4];
+        scores(buffer ^ 1, y);
+        weigh(x, p);
+        if constexpr (kNarrow) {
+          put(0, buffer);
+          fetch(1, tile + 1, entry1);
+        }
+        if (careful && !whole)
+          values_seen(buffer, p, tile * kKeys, present);
+        else
+          values(buffer, p);
+        if constexpr (!careful_now && !kNarrow && D == 128) {
+          __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+          for (int i = 0; i < 2 * kSteps; i++) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+            if (i < 2 * kSteps - 4) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x2, 80 / (2 * kSteps), 0);
+            __builtin_amdgcn_sched_group_barrier(0x400, 32 / (2 * kSteps), 0);
+          }
+          __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+          for (int i = 0; i < 4 * kDims; i++) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+            if (i < 4 * kDims - 3) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+          }
+        }
+        present = present_of(entry1);
+        if (tile + 1 < mine) {
+          whole = mask(y, (tile + 1) * kKeys, present);
+          raise(highest(y));
+        }
+      } else if constexpr (kNarrow) {
+        put(0, buffer);
+        fetch(1, tile + 1, entry1);
+      }
+      if constexpr (kNarrow) put(1, buffer ^ 1);
+      entry1 = entry2, entry2 = entry3;
+    };
+    f32x16 y[2];
+    for (int tile = 0; tile < tiles; tile += 2) {
+      step(Constant<0>{}, tile, x, y);
+      if (tile + 1 < tiles) step(Constant<1>{}, tile + 1, y, x);
+    }
+    __syncthreads();
     }
   };
-  struct No { constexpr operator bool() const { return false; } };
-  struct Yes { constexpr operator bool() const { return true; } };
-  pass(No{});
+  pass(Constant<0>{});
   float check = 0.f;
 #pragma unroll
   for (int d = 0; d < kDims; d++)
 #pragma unroll
     for (int r = 0; r < 16; r++) check = __builtin_fmaf(acc[d][r], 0.f, check);
-  if (__syncthreads_or(real && !(check == 0.f))) pass(Yes{});
+  bool again = __any(real && !(check == 0.f));
+  __syncthreads();
+  if (lane == 0) lds[wave] = again;
+  __syncthreads();
+  again = *reinterpret_cast<const uint32_t*>(lds) != 0;  // the four waves' bytes
+  __syncthreads();
+  if (again) pass(Constant<1>{});
 
+  clear_rest();
   l += __shfl_xor(l, 32);
   float f = l == 0.f ? 0.f : a.value_scale / l;
   if (!real) return;
@@ -350,7 +509,9 @@ hipError_t launch_prompt(const AttendArgs& a, hipStream_t stream) {
   s.negative = a.score_scale < 0;
   // a scale of zero weighs all keys alike, as does one that small, and spares the kernel -inf * 0
   s.a.score_scale = a.score_scale == 0 ? 0x1p-100f : (s.negative ? -a.score_scale : a.score_scale);
-  int64_t items = ((int64_t)a.rows * (a.heads / a.kv_heads)) / kRows + a.requests;
+  auto log2 = [](int x) { return x & (x - 1) ? -1 : __builtin_ctz(x); };
+  s.group = a.heads / a.kv_heads, s.group_log2 = log2(s.group), s.kv_heads_log2 = log2(a.kv_heads);
+  int64_t items = ((int64_t)a.rows * s.group) / kRows + a.requests;
   if (items < 1) items = 1;
   if (items * a.kv_heads >= (1LL << 31)) return hipErrorInvalidValue;
   dim3 grid((unsigned)(items * a.kv_heads));
