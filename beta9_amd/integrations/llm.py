@@ -9,7 +9,10 @@ CausalLM running in bf16 on ROCm, with iteration-level batched greedy/
 sampling decode: pending requests join the active batch at step-group
 boundaries and finished sequences are masked out, so one forward pass per
 step serves every in-flight request (the continuous-batching idea sized
-for a single 288 GB MI355X).
+for a single 288 GB MI355X). ``LLMArgs(kv_cache="paged")`` batches
+continuously over a paged key-value cache instead (llm_paged.py): requests
+join and leave at any step, prompts are packed without padding, and
+attention runs on the kernels of ops/paged.py.
 
 Offline-first: ``model`` may be a local HF directory (loaded with
 from_pretrained) or a synthetic spec — when the path does not exist a
@@ -37,6 +40,12 @@ class LLMArgs:
     max_num_seqs: int = 32  # decode batch width
     tensor_parallel_size: int = 1
     seed: int = 0
+    # "dense": a padded cache for each group of requests; "paged": one cache
+    # in pages for all; "paged_e4m3": the same in 8 bits, values divided by kv_scale
+    kv_cache: str = "dense"
+    kv_page_size: int = 64
+    kv_pages: int = 0  # 0: as many as max_num_seqs requests of max_model_len need
+    kv_scale: float = 0.0625
     # synthetic model dims (used when `model` is not a local directory)
     hidden_size: int = 1024
     intermediate_size: int = 2816
@@ -65,6 +74,7 @@ class _Request:
         self.max_tokens = max_tokens
         self.temperature = temperature
         self.out_ids: List[int] = []
+        self.error: Optional[Exception] = None
         self.done = asyncio.Event()
         self.created = time.time()
 
@@ -108,10 +118,17 @@ class LLMEngine:
             self.model = LlamaForCausalLM(cfg).to(self.dtype)
         self.model = self.model.to(self.device).eval()
         self.eos_id = getattr(self.tokenizer, "eos_token_id", None)
+        from .llm_paged import KINDS, PagedDecoder
+
+        if self.args.kv_cache not in KINDS:
+            raise ValueError(f"kv_cache must be one of {KINDS}, is {self.args.kv_cache!r}")
+        self.paged: Optional[PagedDecoder] = None
+        if self.args.kv_cache != "dense":
+            self.paged = PagedDecoder(self.model, self.args, self.eos_id, self.dtype, self.device)
 
     async def start(self) -> None:
         if self._task is None:
-            self._task = asyncio.create_task(self._loop())
+            self._task = asyncio.create_task(self._loop() if self.paged is None else self._loop_paged())
 
     async def stop(self) -> None:
         if self._task is not None:
@@ -128,6 +145,8 @@ class LLMEngine:
         req = _Request(ids, max_tokens, temperature)
         await self._queue.put(req)
         await req.done.wait()
+        if req.error is not None:
+            raise req.error
         return self.tokenizer.decode(req.out_ids)
 
     async def _loop(self) -> None:
@@ -138,6 +157,18 @@ class LLMEngine:
                 batch.append(self._queue.get_nowait())
             await asyncio.get_event_loop().run_in_executor(None, self._decode_group, batch)
             for r in batch:
+                r.done.set()
+
+    async def _loop_paged(self) -> None:
+        while True:
+            arrived = [] if self.paged.active else [await self._queue.get()]
+            while not self._queue.empty():
+                arrived.append(self._queue.get_nowait())
+            try:
+                ended = await asyncio.get_event_loop().run_in_executor(None, self.paged.step, arrived)
+            except Exception as e:
+                ended = self.paged.fail(e)
+            for r in ended:
                 r.done.set()
 
     def _decode_group(self, batch: List[_Request]) -> None:

@@ -1,0 +1,208 @@
+"""Continuous batching for LLMEngine over the paged key-value cache.
+
+With ``LLMArgs(kv_cache="paged")`` (or ``"paged_e4m3"``: 8-bit pages) the
+engine keeps one PagedKVCache for all requests instead of a dense, padded
+cache for each group: a request joins at any step as soon as a row and its
+pages are free, its prompt is read in one packed pass without padding, every
+decode step runs all active requests, and its pages go back when it ends.
+
+The model's layers are transformers' own; only their attention is replaced,
+through its AttentionInterface: the new keys and values go into the pages
+(ops/paged.py write_kv), and decode_attention or prompt_attention reads them.
+"""
+
+from __future__ import annotations
+
+import threading
+from typing import Any, List, Optional
+
+NAME = "beta9_paged"
+KINDS = ("dense", "paged", "paged_e4m3")
+
+
+class Step:
+    """What one forward pass tells its layers' attention."""
+
+    def __init__(self, cache, plan, active=None):
+        self.cache, self.plan, self.active = cache, plan, active  # active: of a decode step's rows
+
+
+def attention(module, query, key, value, attention_mask, scaling=None, paged_step=None, **kwargs):
+    """transformers' attention signature; query [1, heads, tokens, dim]."""
+    if paged_step is None:
+        raise RuntimeError("this model's attention runs on a paged cache: call it through the engine")
+    if kwargs.get("sliding_window") is not None or kwargs.get("softcap") is not None or kwargs.get("s_aux") is not None:
+        raise ValueError("the paged cache serves full attention only, without windows, caps or sinks")
+    step, layer = paged_step, module.layer_idx
+    cache, plan = step.cache, step.plan
+    q, k, v = (x[0].transpose(0, 1) for x in (query, key, value))  # [tokens, heads, dim]
+    cache.write(layer, k, v, plan)
+    if step.active is None:
+        out = cache.prompt(layer, q, plan, scaling)
+    else:
+        out = cache.decode(layer, q, plan, scaling, step.active)
+    return out.unsqueeze(0), None
+
+
+def register() -> str:
+    """Makes the attention known to transformers; returns its name there."""
+    from transformers import AttentionInterface, AttentionMaskInterface
+
+    AttentionInterface.register(NAME, attention)
+    AttentionMaskInterface.register(NAME, lambda *args, **kwargs: None)  # lengths and positions say it all
+    return NAME
+
+
+class PagedDecoder:
+    """Rows, pages and steps of one engine's model."""
+
+    def __init__(self, model, args, eos_id: Optional[int], dtype, device: str):
+        import torch
+
+        from ..ops.paged import MAX_HEAD_DIM, PagedKVCache
+
+        cfg = model.config
+        heads = cfg.num_attention_heads
+        dim = getattr(cfg, "head_dim", None) or cfg.hidden_size // heads
+        kv_heads = getattr(cfg, "num_key_value_heads", None) or heads
+        kinds = set(getattr(cfg, "layer_types", None) or ["full_attention"])
+        if dim % 8 or dim > MAX_HEAD_DIM or kinds != {"full_attention"}:
+            raise ValueError(
+                f"kv_cache={args.kv_cache!r} needs full attention in every layer and a head dim that is a "
+                f"multiple of 8 up to {MAX_HEAD_DIM}; this model has {sorted(kinds)} and {dim}"
+            )
+        model.set_attn_implementation(register())
+        self.model, self.args, self.eos_id, self.device = model, args, eos_id, device
+        size = args.kv_page_size
+        pages = args.kv_pages or args.max_num_seqs * -(-args.max_model_len // size)
+        e4m3 = args.kv_cache == "paged_e4m3"
+        self.cache = PagedKVCache(
+            cfg.num_hidden_layers, kv_heads, dim, pages, size, args.max_num_seqs, args.max_model_len,
+            torch.float8_e4m3fn if e4m3 else dtype, device,
+            *((args.kv_scale, args.kv_scale) if e4m3 else ()),
+        )
+        self.rows: List[Any] = [None] * args.max_num_seqs  # request of each row
+        self.lens = [0] * args.max_num_seqs  # tokens held, as the GPU has them
+        self.reserved = [0] * args.max_num_seqs  # pages a row may come to hold
+        self.waiting: List[Any] = []
+        self._ended: List[Any] = []
+        self._freed: List[int] = []
+        # a step whose loop was stopped runs on in its thread; the next one waits for it
+        self._lock = threading.Lock()
+
+    @property
+    def active(self) -> bool:
+        return any(r is not None for r in self.rows) or bool(self.waiting)
+
+    def _most(self, req) -> int:
+        """Tokens the request can come to hold: its last one is never written."""
+        return min(len(req.prompt_ids) + req.max_tokens - 1, self.args.max_model_len)
+
+    def _admit(self) -> List[int]:
+        """Rows of the waiting requests that start now, in their order."""
+        started = []
+        while self.waiting:
+            req = self.waiting[0]
+            if req.max_tokens <= 0 or not req.prompt_ids:
+                if not req.prompt_ids:
+                    req.error = ValueError("the prompt has no tokens")
+                self._ended.append(self.waiting.pop(0))
+                continue
+            pages = self.cache.pages_for(self._most(req))
+            if len(req.prompt_ids) > self.args.max_model_len or pages > self.cache.pages:
+                req.error = ValueError(
+                    f"a request of {len(req.prompt_ids)} + {req.max_tokens} tokens does not fit the cache: "
+                    f"{self.args.max_model_len} tokens a row, {self.cache.pages} pages of {self.cache.page_size}"
+                )
+                self._ended.append(self.waiting.pop(0))
+                continue
+            free = [r for r, q in enumerate(self.rows) if q is None]
+            if not free or sum(self.reserved) + pages > self.cache.pages:
+                break  # first come, first served
+            row = free[0]
+            self.rows[row], self.reserved[row], self.lens[row] = self.waiting.pop(0), pages, 0
+            started.append(row)
+        return started
+
+    def _forward(self, rows: List[int], ids: List[int], new: List[int], decode: bool) -> List[int]:
+        """One pass over the packed tokens of `rows`; each row's next token."""
+        import torch
+
+        put = lambda x, t: torch.tensor(x, dtype=t, device=self.device)  # noqa: E731
+        new_lens = [0] * len(self.rows)
+        for row, n in zip(rows, new):
+            new_lens[row] = n
+            self.lens[row] += n
+        plan = self.cache.plan(put(new_lens, torch.int32), len(ids))
+        step = Step(self.cache, plan, self.cache.active(plan, put(rows, torch.long)) if decode else None)
+        ends = put([sum(new[: i + 1]) - 1 for i in range(len(new))], torch.long)
+        logits = self.model(
+            input_ids=put([ids], torch.long),
+            position_ids=plan.positions.long().unsqueeze(0),
+            use_cache=False,
+            logits_to_keep=ends,
+            paged_step=step,
+        ).logits[0].float()
+        tokens = logits.argmax(-1).tolist()
+        for i, row in enumerate(rows):
+            t = self.rows[row].temperature
+            if t > 0:
+                tokens[i] = int(torch.multinomial(torch.softmax(logits[i] / t, dim=-1), 1).item())
+        return tokens
+
+    def _take(self, rows: List[int], tokens: List[int]) -> None:
+        for row, token in zip(rows, tokens):
+            req = self.rows[row]
+            req.out_ids.append(token)
+            full = self.lens[row] >= self.args.max_model_len
+            if (self.eos_id is not None and token == self.eos_id) or len(req.out_ids) >= req.max_tokens or full:
+                self._ended.append(req)
+                self.rows[row] = None
+                self._freed.append(row)
+
+    def fail(self, error: Exception) -> List[Any]:
+        with self._lock:
+            return self._fail(error)
+
+    def _fail(self, error: Exception) -> List[Any]:
+        """After a step that raised: ends every request with its error, and
+        starts again with an empty cache."""
+        import torch
+
+        ended = [r for r in self.rows if r is not None] + self.waiting
+        for req in ended:
+            req.error = error
+        ended = ended + [r for r in self._ended if r not in ended]
+        n = len(self.rows)
+        self.rows, self.lens, self.reserved, self.waiting = [None] * n, [0] * n, [0] * n, []
+        self.cache.release(torch.ones(n, dtype=torch.bool, device=self.device))
+        return ended
+
+    def step(self, arrived: List[Any]) -> List[Any]:
+        """Takes in what arrived, reads the prompts that fit, decodes one
+        token of every active request; returns the requests that ended."""
+        with self._lock:
+            return self._step(arrived)
+
+    def _step(self, arrived: List[Any]) -> List[Any]:
+        import torch
+
+        self._ended, self._freed = [], []
+        self.waiting.extend(arrived)
+        with torch.inference_mode():
+            started = self._admit()
+            if started:
+                prompts = sorted(started)  # the plan packs by row
+                ids = [self.rows[r].prompt_ids for r in prompts]
+                self._take(prompts, self._forward(prompts, sum(ids, []), [len(i) for i in ids], False))
+            rows = [r for r, q in enumerate(self.rows) if q is not None]
+            if rows:
+                last = [self.rows[r].out_ids[-1] for r in rows]
+                self._take(rows, self._forward(rows, last, [1] * len(rows), True))
+            if self._freed:
+                done = torch.zeros(len(self.rows), dtype=torch.bool)
+                done[self._freed] = True
+                self.cache.release(done.to(self.device))
+                for row in self._freed:
+                    self.reserved[row] = self.lens[row] = 0
+        return self._ended

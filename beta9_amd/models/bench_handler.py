@@ -130,10 +130,18 @@ class _CPUModel:
         return {"ms": (time.perf_counter() - t0) * 1000, "tflops": 0.0, "checksum": float(x.abs().mean())}
 
 
-def infer(tokens: int = 256, **kwargs) -> Dict[str, Any]:
+def infer(tokens: int = 256, decode_steps: int = 0, requests: int = 32, **kwargs) -> Dict[str, Any]:
+    """One forward of ``tokens`` tokens; with decode_steps (transformer
+    model), prompts of ``tokens`` tokens for ``requests`` requests and that
+    many decode steps over a paged key-value cache."""
     if _model is None:
         load()
-    r = _model.infer(batch_tokens=int(tokens))
+    if decode_steps:
+        if not hasattr(_model, "infer_decode"):
+            raise ValueError("decode_steps needs the transformer model (B9_BENCH_MODEL=transformer)")
+        r = _model.infer_decode(int(requests), int(tokens), int(decode_steps))
+    else:
+        r = _model.infer(batch_tokens=int(tokens))
     r["load"] = _load_info
     return r
 

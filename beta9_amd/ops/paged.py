@@ -213,7 +213,9 @@ class PagedKVCache:
             cache.write(layer, k, v, plan)
             o = cache.decode(layer, q, plan)      # or cache.prompt(...)
 
-    and ``cache.release(done)`` when requests end. plan, write, decode and
+    and ``cache.release(done)`` when requests end. ``decode`` takes one row
+    of q for each request of the cache; if only some have a new token, their
+    rows alone, with ``active=cache.active(plan, rows)``. plan, write, decode and
     prompt may be captured into a graph; its replays read and advance the
     same state. Steps of one cache run in order, on one stream at a time."""
 
@@ -271,9 +273,22 @@ class PagedKVCache:
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, plan: StepPlan) -> None:
         write_kv(k, v, self.k[layer], self.v[layer], plan.slots, self.k_scale, self.v_scale)
 
-    def decode(self, layer: int, q: torch.Tensor, plan: StepPlan, scale: Optional[float] = None) -> torch.Tensor:
+    def active(self, plan: StepPlan, rows: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Tables and lengths of the requests ``rows`` (int64, ascending as
+        the plan packs them), for all layers of a decode step."""
+        return self.tables[rows], plan.kv_lens[rows]
+
+    def decode(
+        self,
+        layer: int,
+        q: torch.Tensor,
+        plan: StepPlan,
+        scale: Optional[float] = None,
+        active: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
+    ) -> torch.Tensor:
+        tables, kv_lens = (self.tables, plan.kv_lens) if active is None else active
         return decode_attention(
-            q, self.k[layer], self.v[layer], self.tables, plan.kv_lens, scale, self.k_scale, self.v_scale
+            q, self.k[layer], self.v[layer], tables, kv_lens, scale, self.k_scale, self.v_scale
         )
 
     def prompt(self, layer: int, q: torch.Tensor, plan: StepPlan, scale: Optional[float] = None) -> torch.Tensor:

@@ -1,0 +1,156 @@
+"""The LLM engine over the paged key-value cache."""
+
+import asyncio
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytest.importorskip("transformers")
+
+from beta9_amd.integrations import LLMArgs  # noqa: E402
+from beta9_amd.integrations.llm import LLMEngine, _Request  # noqa: E402
+
+
+def args(**more):
+    base = dict(
+        hidden_size=64, intermediate_size=128, num_hidden_layers=2, num_attention_heads=4, max_model_len=128,
+        max_num_seqs=3, kv_page_size=16,
+    )
+    return LLMArgs(**{**base, **more})
+
+
+def ids_of(engine, prompts, steps):
+    """Greedy tokens of all prompts at once, by the engine's own decode."""
+
+    async def main():
+        reqs = [_Request(engine.tokenizer.encode(p), n, 0.0) for p, n in zip(prompts, steps)]
+        engine._queue = asyncio.Queue()  # a queue belongs to one event loop
+        await engine.start()
+        for r in reqs:
+            await engine._queue.put(r)
+        for r in reqs:
+            await asyncio.wait_for(r.done.wait(), 120)
+        await engine.stop()
+        return [r.out_ids for r in reqs], [r.error for r in reqs]
+
+    return asyncio.run(main())
+
+
+PROMPTS = ["hello", "a longer prompt than the others, over three pages of sixteen", "x", "abc" * 9, "last one", "q" * 40]
+STEPS = [5, 20, 1, 12, 33, 7]
+
+
+def alone(engine, prompt, steps):
+    """The same model without any cache, in 64 bits: the whole sequence again for each token."""
+    engine.model.set_attn_implementation("eager")
+    model = engine.model.double()
+    ids = engine.tokenizer.encode(prompt)
+    out = []
+    with torch.inference_mode():
+        for _ in range(steps):
+            logits = model(input_ids=torch.tensor([ids], device=engine.device), use_cache=False).logits[0, -1]
+            out.append(int(logits.argmax()))
+            ids = ids + out[-1:]
+            if out[-1] == engine.eos_id:
+                break
+    return out
+
+
+def test_paged_tokens_are_the_models():
+    """More requests than rows, joining as rows become free; each gets the tokens it would get alone."""
+    if torch.cuda.is_available():
+        pytest.skip("32-bit caches are the CPU's")
+    got, errors = ids_of(LLMEngine(args(kv_cache="paged")), PROMPTS, STEPS)
+    assert errors == [None] * len(PROMPTS)
+    reference = LLMEngine(args())
+    for prompt, steps, tokens in zip(PROMPTS, STEPS, got):
+        assert tokens == alone(reference, prompt, steps)
+
+
+def test_paged_with_few_pages_and_small_rows():
+    """Requests wait for pages; one that can never fit is refused, and the others go on. The second prompt's 61 tokens and
+    19 of the 20 that it asks for (the last is not held) fill five pages of 16 exactly."""
+    engine = LLMEngine(args(kv_cache="paged", kv_pages=5))
+    got, errors = ids_of(engine, PROMPTS, STEPS)
+    assert errors == [None] * len(PROMPTS)
+    assert [len(t) <= n for t, n in zip(got, STEPS)] == [True] * len(PROMPTS)
+    engine = LLMEngine(args(kv_cache="paged", kv_pages=4))
+    got, errors = ids_of(engine, PROMPTS, STEPS)
+    assert isinstance(errors[1], ValueError) and errors[:1] + errors[2:] == [None] * 5
+    assert engine.paged.cache.free_count.tolist() == [4] and engine.paged.cache.lens.tolist() == [0, 0, 0]
+    assert sorted(engine.paged.cache.free_pages.tolist()) == list(range(4))
+    # a request ends where its row does
+    engine = LLMEngine(args(kv_cache="paged", max_model_len=32))
+    got, errors = ids_of(engine, ["hello"], [100])
+    assert errors == [None] and len(got[0]) <= 32 - 6 + 1
+    if engine.eos_id not in got[0]:
+        assert len(got[0]) == 32 - 6 + 1
+
+
+def test_paged_e4m3_and_sampling_run():
+    engine = LLMEngine(args(kv_cache="paged_e4m3"))
+    assert engine.paged.cache.k.dtype == torch.float8_e4m3fn
+
+    async def main():
+        try:
+            return await asyncio.gather(*[engine.generate(p, 6, temperature=0.8) for p in PROMPTS])
+        finally:
+            await engine.stop()
+
+    assert all(isinstance(t, str) for t in asyncio.run(main()))
+
+
+def test_paged_refusals():
+    with pytest.raises(ValueError, match="kv_cache"):
+        LLMEngine(args(kv_cache="none"))
+    with pytest.raises(ValueError, match="head dim"):
+        LLMEngine(args(kv_cache="paged", hidden_size=48, num_attention_heads=4))
+    with pytest.raises(ValueError, match="page_size"):
+        LLMEngine(args(kv_cache="paged", kv_page_size=17))
+    engine = LLMEngine(args(kv_cache="paged"))
+    got, errors = ids_of(engine, ["hello", "ok"], [0, 2])
+    assert got[0] == [] and errors == [None, None] and len(got[1]) in (1, 2)
+    with pytest.raises(RuntimeError, match="engine"):
+        engine.model(input_ids=torch.tensor([[1, 2]], device=engine.device), use_cache=False)
+
+
+def test_a_step_that_raises_ends_its_requests_and_no_more():
+    engine = LLMEngine(args(kv_cache="paged"))
+    whole, failed = engine.paged._forward, []
+
+    def forward(*a):
+        if not failed:
+            failed.append(True)
+            whole(*a)
+            raise RuntimeError("planned")
+        return whole(*a)
+
+    engine.paged._forward = forward
+    _, errors = ids_of(engine, ["hello", "there"], [3, 3])
+    assert any(isinstance(e, RuntimeError) for e in errors)
+    got, errors = ids_of(engine, ["hello"], [3])
+    assert errors == [None] and 1 <= len(got[0]) <= 3
+    assert engine.paged.cache.free_count.tolist() == [engine.paged.cache.pages]
+
+
+@pytest.mark.gpu
+@pytest.mark.skipif(not torch.cuda.is_available(), reason="needs MI355X")
+@pytest.mark.parametrize("kind", ["paged", "paged_e4m3"])
+@pytest.mark.parametrize("heads", [4, 2])  # head dims of 64 and 128
+def test_paged_on_the_gpu(kind, heads):
+    """bf16: the first token of each prompt is within rounding of the best one in 64 bits."""
+    more = dict(hidden_size=256, intermediate_size=512, num_attention_heads=heads, kv_page_size=32)
+    engine = LLMEngine(args(kv_cache=kind, **more))
+    got, errors = ids_of(engine, PROMPTS, STEPS)
+    assert errors == [None] * len(PROMPTS)
+    assert engine.paged.cache.free_count.tolist() == [engine.paged.cache.pages]
+    model = LLMEngine(args(**more)).model.double()
+    model.set_attn_implementation("eager")
+    for prompt, tokens in zip(PROMPTS, got):
+        ids = torch.tensor([engine.tokenizer.encode(prompt)], device="cuda")
+        with torch.inference_mode():
+            logits = model(input_ids=ids, use_cache=False).logits[0, -1]
+        # bf16 rounds what each of the 2 x 7 products and 4 sums of two layers gives: logits may be off by their spread
+        # times a few 2^-8, e4m3 keys and values by 2^-4 of theirs; a wrong row or page moves them by the whole spread
+        off = {"paged": 0.25, "paged_e4m3": 0.75}[kind]
+        assert float(logits.max() - logits[tokens[0]]) <= off * float(logits.std())

@@ -651,3 +651,254 @@ def test_tensors_of_two_devices_are_refused():
         paged.decode_attention(**{**args, "q": args["q"].cpu()})
     with pytest.raises(TypeError):
         paged.decode_attention(**{n: x.float() if x.is_floating_point() else x for n, x in args.items()})
+
+
+# -- the operators together -------------------------------------------------
+
+
+class Dense:
+    """A request's keys, values and last output in 64 bits, beside the paged cache."""
+
+    def __init__(self, layers, kv_heads, dim):
+        self.k = [torch.zeros((0, kv_heads, dim), dtype=torch.float64) for _ in range(layers)]
+        self.v = [torch.zeros((0, kv_heads, dim), dtype=torch.float64) for _ in range(layers)]
+
+
+@both
+@pytest.mark.parametrize("kind,cached,dim", [("bf16", "bf16", 64), ("fp16", "fp16", 128), ("bf16", "e4m3", 128), ("bf16", "bf16", 80)])
+def test_requests_come_and_go(device, kind, cached, dim):
+    """A server's steps on one cache: prompts in parts, decoding, ends, rows and pages used again, a pool that runs short.
+    Every output is compared with attention over the request's own keys and values, as the cache holds them."""
+    rng = random.Random(dim)
+    gen = torch.Generator().manual_seed(dim)
+    layers, heads, kv_heads, rows, page = 2, 4, 2, 6, 16
+    scales = (0.03125, 0.0625) if cached == "e4m3" else (1.0, 1.0)
+    cache = paged.PagedKVCache(layers, kv_heads, dim, 17, page, rows, 200, TYPES[cached], device, *scales)
+    dense = [Dense(layers, kv_heads, dim) for _ in range(rows)]
+    refused = 0
+    for step in range(24):
+        decode = step % 3 != 0
+        held = cache.lens.tolist()
+        if decode:
+            new = [1] * rows
+        else:
+            new = [rng.choice([0, rng.randint(1, 70)]) for _ in range(rows)]
+        total = sum(new)
+        plan = cache.plan(ints(new, device), total + (0 if decode else 5))
+        served = [n > 0 and k > 0 for n, k in zip(new, plan.kv_lens.tolist())]
+        refused += sum(n > 0 and not s for n, s in zip(new, served))
+        assert cache.lens.tolist() == [h + (n if s else 0) for h, n, s in zip(held, new, served)]
+        cu = plan.cu_new.tolist()
+        for layer in range(layers):
+            fused = torch.randn((plan.slots.shape[0], heads + 2 * kv_heads, dim), generator=gen).to(TYPES[kind]).to(device)
+            q, k, v = fused[:, :heads], fused[:, heads : heads + kv_heads], fused[:, heads + kv_heads :]
+            cache.write(layer, k, v, plan)
+            out = (cache.decode if decode else cache.prompt)(layer, q, plan)
+            for r in range(rows):
+                part = slice(cu[r], cu[r + 1])
+                if not served[r]:
+                    assert (out[part] == 0).all()
+                    continue
+                d = dense[r]
+                for x, have, scale in ((k, d.k, scales[0]), (v, d.v, scales[1])):
+                    have[layer] = torch.cat([have[layer], values_of(cache_like(x[part].cpu(), TYPES[cached], scale), scale)])
+                n = len(d.k[layer])
+                # one page that holds all of the request's tokens
+                whole = (d.k[layer][None].transpose(1, 2).contiguous(), d.v[layer][None].transpose(1, 2).contiguous())
+                want, off = attention_oracle(q[part], *whole, [[0]], [n], [0, new[r]], dim**-0.5, 1.0, 1.0)
+                assert ((out[part].cpu().double() - want).abs() <= off).all()
+            assert (out[cu[-1] :] == 0).all()
+        # no page has two owners
+        used = [cache.tables[r, : cache.pages_for(n)].tolist() for r, n in enumerate(cache.lens.tolist())]
+        stack = cache.free_pages[: int(cache.free_count)].tolist()
+        assert sorted(sum(used, []) + stack) == list(range(cache.pages))
+        if step % 4 == 3:
+            done = [rng.random() < 0.5 for _ in range(rows)]
+            cache.release(torch.tensor(done, device=device))
+            for r in range(rows):
+                if done[r]:
+                    dense[r] = Dense(layers, kv_heads, dim)
+    assert refused  # the pool did run short
+
+
+@both
+def test_cache_arguments(device):
+    with pytest.raises(ValueError):
+        paged.PagedKVCache(1, 1, 64, 4, page_size=20, device=device)
+    with pytest.raises(ValueError):
+        paged.PagedKVCache(0, 1, 64, 4, device=device)
+    cache = paged.PagedKVCache(1, 2, 64, 4, 16, 2, 40, device=device)
+    assert cache.tables.shape == (2, 3) and cache.pages == 4 and cache.pages_for(17) == 2 and cache.k.dtype == torch.bfloat16
+
+
+@both
+def test_transformer_model_over_the_cache(device):
+    """Prompts in two parts and a decode step give what the whole sequences give at once."""
+    from beta9_amd.models.transformer import TransformerServingModel
+
+    torch.manual_seed(0)
+    # 4 heads of 64; a scale that keeps the random layers' outputs near their inputs' size
+    model = TransformerServingModel(hidden=256, inter=512, layers=2, n_heads=4, n_kv_heads=2, device=device)
+    for b in model.blocks:
+        for w in (b.attn_norm, b.mlp_norm):
+            w.fill_(1.0)
+    lens = [70, 1, 33]
+    x = [torch.randn((n + 1, 256), device=device).to(torch.bfloat16) for n in lens]
+    cache = model.new_cache(requests=3, max_len=100, page_size=16)
+    first = [40, 0, 33]
+    got = [[], [], []]
+    for part in ([(0, f) for f in first], [(f, n) for f, n in zip(first, lens)]):
+        new = ints([b - a for a, b in part], device)
+        y = model.prompt(torch.cat([v[a:b] for v, (a, b) in zip(x, part)]), new, cache)
+        for r, piece in enumerate(y.split([b - a for a, b in part])):
+            got[r].append(piece)
+    y = model.decode(torch.stack([v[n] for v, n in zip(x, lens)]), cache)
+    for r in range(3):
+        got[r].append(y[r : r + 1])
+    for r in range(3):
+        whole = x[r]
+        for b in model.blocks:
+            whole = b.forward(whole)
+        a, b = torch.cat(got[r]).double(), whole.double()
+        # both round attention, projections, norms and sums to bf16, in 2 layers of 9 operations each: 36 roundings of
+        # half a step, 2^-8, that add up as independent ones; the maximum over 256 x 71 values is within 5 deviations
+        assert float((a - b).abs().max() / b.std()) <= 5 * (2 * 2 * 9) ** 0.5 * 2**-8
+
+
+# -- streams, graphs, threads -----------------------------------------------
+
+gpu = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(), reason="needs MI355X")]
+
+
+class Loop:
+    """A decode step of two layers over a cache of its own, its inputs changed from outside."""
+
+    def __init__(self, seed, rows=5, heads=8, kv_heads=2, dim=128):
+        self.gen = torch.Generator().manual_seed(seed)
+        self.rows, self.heads, self.kv_heads, self.dim = rows, heads, kv_heads, dim
+        self.cache = paged.PagedKVCache(2, kv_heads, dim, 40, 16, rows, 700, device="cuda")
+        self.one = torch.ones(rows, dtype=torch.int32, device="cuda")
+        self.fused = torch.zeros((2, rows, heads + 2 * kv_heads, dim), dtype=torch.bfloat16, device="cuda")
+        n = [3, 17, 0, 40, 1]
+        plan = self.cache.plan(ints(n, "cuda"), sum(n))
+        x = torch.randn((2, sum(n), 2 * kv_heads, dim), generator=self.gen).to(torch.bfloat16).cuda()
+        for layer in range(2):
+            self.cache.write(layer, x[layer, :, :kv_heads], x[layer, :, kv_heads:], plan)
+
+    def fresh(self):
+        self.fused.copy_(torch.randn(self.fused.shape, generator=self.gen))
+
+    def step(self):
+        h, kv = self.heads, self.kv_heads
+        plan = self.cache.plan(self.one, self.rows)
+        out = []
+        for layer in range(2):
+            x = self.fused[layer]
+            self.cache.write(layer, x[:, h : h + kv], x[:, h + kv :], plan)
+            out.append(self.cache.decode(layer, x[:, :h], plan))
+            out.append(self.cache.prompt(layer, x[:, :h], plan))
+        return out + list(plan)
+
+    def state(self):
+        return [self.cache.lens, self.cache.free_count, self.cache.tables, self.cache.k, self.cache.v]
+
+
+def captured(loop):
+    """The step in a graph, and its outputs; the state is as before the capture."""
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        out = loop.step()
+    return graph, out
+
+
+class TestOnTheGpu:
+    pytestmark = gpu
+
+    def test_two_captured_steps_replayed_in_turn(self):
+        """Two caches' steps in graphs of their own, an eager twin of each beside them, many replays with other work and
+        synchronizations between: every replay gives what the eager step gives, bit by bit."""
+        loops, twins = [Loop(1), Loop(2)], [Loop(1), Loop(2)]
+        for x in twins:
+            x.fresh(), x.step()  # code is loaded before the capture
+        for x in loops:
+            x.fresh(), x.step()
+        graphs = [captured(x) for x in loops]
+        for turn in range(8):
+            for which in (0, 1) if turn % 2 else (1, 0):
+                loop, twin, (graph, out) = loops[which], twins[which], graphs[which]
+                loop.fresh(), twin.fresh()
+                graph.replay()
+                want = twin.step()
+                torch.randn((512, 512), device="cuda").sum()
+                if turn % 3 == 0:
+                    torch.cuda.synchronize()
+                for a, b in zip(out + loop.state(), want + twin.state()):
+                    assert torch.equal(a, b)
+        assert loops[0].cache.lens.tolist() == [3 + 9, 17 + 9, 9, 40 + 9, 1 + 9]
+
+    def test_calls_on_several_streams_at_once(self):
+        """The same calls on three streams, enqueued without waiting, give the bits of the calls one by one."""
+        gen = torch.Generator().manual_seed(9)
+        jobs = []
+        for lens, heads, kv_heads, dim in (([900, 30, 2000], 8, 2, 128), ([64] * 30, 4, 4, 64), ([5000], 16, 1, 128)):
+            cache = make_cache(gen, lens, kv_heads, dim, 16, "bf16", "bf16", "cuda")
+            q = torch.randn((sum(min(n, 100) for n in lens), heads, dim), generator=gen).to(torch.bfloat16).cuda()
+            cu = [0]
+            for n in lens:
+                cu.append(cu[-1] + min(n, 100))
+            jobs.append((q, cache, lens, cu))
+        calls = lambda q, cache, lens, cu: (run_decode(q[: len(lens)], cache, lens), run_prompt(q, cache, lens, cu))  # noqa: E731
+        want = [calls(*j) for j in jobs]
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in jobs]
+        got = []
+        for _ in range(10):
+            for stream, job in zip(streams, jobs):
+                stream.wait_stream(torch.cuda.current_stream())
+                with torch.cuda.stream(stream):
+                    got.append(calls(*job))
+        torch.cuda.synchronize()
+        for i, pair in enumerate(got):
+            for a, b in zip(pair, want[i % len(jobs)]):
+                assert torch.equal(a, b)
+
+    def test_runs_are_the_same_bit_by_bit(self):
+        gen = torch.Generator().manual_seed(10)
+        lens = [3000, 1, 700, 0, 2500]
+        cache = make_cache(gen, lens, 2, 128, 64, "bf16", "e4m3", "cuda")
+        q = torch.randn((5, 8, 128), generator=gen).to(torch.bfloat16).cuda()
+        first = run_decode(q, cache, lens)
+        for _ in range(5):
+            assert torch.equal(run_decode(q, cache, lens), first)
+
+    def test_slots_past_two_to_the_31_bytes(self):
+        """A cache of more than 4 GB a side: offsets pass 32 bits."""
+        pages, page, dim = 140_000, 64, 128
+        k = torch.empty((pages, 2, page, dim), dtype=torch.bfloat16, device="cuda")
+        v = torch.empty_like(k)
+        gen = torch.Generator().manual_seed(11)
+        rows = [pages - 1, 0, pages - 2, 70_001]
+        n = 250
+        x = torch.randn((n, 6, dim), generator=gen).to(torch.bfloat16).cuda()
+        slots = torch.cat([torch.arange(p * page, (p + 1) * page, dtype=torch.int32) for p in rows])[:n].cuda()
+        paged.write_kv(x[:, 2:4], x[:, 4:], k, v, slots)
+        small_k = torch.stack([k[p] for p in rows])
+        small_v = torch.stack([v[p] for p in rows])
+        near, far = [[0, 1, 2, 3]], [rows]
+        q = x[:, :2].repeat(1, 2, 1)
+        for run, more in ((run_decode, ()), (run_prompt, ([0, n],))):
+            rows_of_q = q[:1] if run is run_decode else q
+            small = run(rows_of_q, (small_k, small_v, near, (1.0, 1.0)), [n], *more)
+            check_attention(small, rows_of_q, (small_k, small_v, near, (1.0, 1.0)), [n], more[0] if more else [0, 1])
+            assert torch.equal(run(rows_of_q, (k, v, far, (1.0, 1.0)), [n], *more), small)
+
+    def test_another_current_device(self):
+        if torch.cuda.device_count() < 2:
+            pytest.skip("one GPU")
+        loop = Loop(3)
+        loop.fresh()
+        with torch.cuda.device(1):
+            out = loop.step()
+        assert all(t.device == loop.fused.device for t in out)
