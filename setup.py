@@ -14,8 +14,8 @@ from torch.utils.cpp_extension import BuildExtension, CUDAExtension  # noqa: E40
 CSRC = os.path.join(os.path.dirname(os.path.abspath(__file__)), "beta9_amd", "ops", "csrc")
 
 ext_flags = ["-O3", "-std=c++17"]
-# packed fp32 arithmetic is left out of the paged cache's kernels: some of its forms have given wrong results on MI355X
-paged_flags = ext_flags + ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+# packed fp32 arithmetic is left out of all HIP code: some of its forms have given wrong results on MI355X
+hip_flags = ext_flags + ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 setup(
     name="beta9-amd",
@@ -26,12 +26,12 @@ setup(
         CUDAExtension(
             name="beta9_amd.ops._hipsnap_ext",
             sources=[os.path.join(CSRC, "hipsnap.hip")],
-            extra_compile_args={"cxx": ext_flags, "nvcc": ext_flags},
+            extra_compile_args={"cxx": ext_flags, "nvcc": hip_flags},
         ),
         CUDAExtension(
             name="beta9_amd.ops._gemm_ext",
             sources=[os.path.join(CSRC, "gemm.hip")],
-            extra_compile_args={"cxx": ext_flags, "nvcc": ext_flags},
+            extra_compile_args={"cxx": ext_flags, "nvcc": hip_flags},
         ),
         CUDAExtension(
             name="beta9_amd.ops._paged_ext",
@@ -39,7 +39,7 @@ setup(
                 os.path.join(CSRC, "paged", name)
                 for name in ("bind.cpp", "tables.hip", "write.hip", "rows.hip", "decode.hip", "prompt.hip")
             ],
-            extra_compile_args={"cxx": ext_flags, "nvcc": paged_flags},
+            extra_compile_args={"cxx": ext_flags, "nvcc": hip_flags},
         ),
     ],
     cmdclass={"build_ext": BuildExtension.with_options(no_python_abi_suffix=True)},
