@@ -75,6 +75,14 @@ void check_table(const Tensor& tables, const Tensor& like, int64_t page_size) {
 
 void check_scale(double x, const char* name) { REQUIRE(std::isfinite(x) && x > 0, name, " must be a positive number, is ", x); }
 
+// A view of n values of a one-dimensional buffer, made directly: six of them by the dispatcher cost more than the launch.
+Tensor part_of(const Tensor& buffer, int64_t first, int64_t n) {
+  Tensor t = at::detail::make_tensor<at::TensorImpl>(c10::Storage(buffer.storage()), buffer.key_set(), buffer.dtype());
+  t.unsafeGetTensorImpl()->set_storage_offset(first);
+  t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+  return t;
+}
+
 std::vector<Tensor> plan_step(const Tensor& tables, const Tensor& lens, const Tensor& new_lens, const Tensor& free_pages,
                               const Tensor& free_count, int64_t page_size, int64_t num_tokens) {
   paged::PlanArgs a;
@@ -91,18 +99,19 @@ std::vector<Tensor> plan_step(const Tensor& tables, const Tensor& lens, const Te
   REQUIRE(free_pages.size(0) * page_size < (1LL << 31), "the cache must have fewer than 2^31 slots");
   REQUIRE(num_tokens >= 0 && num_tokens < (1LL << 31), "num_tokens must be 0 or more and fit 31 bits, is ", num_tokens);
   c10::DeviceGuard guard(tables.device());
-  auto options = tables.options();
-  Tensor token = at::empty({2, num_tokens}, options), state = at::empty({n + 1}, options);
-  Tensor cu = at::empty({n + 1}, options), kv = at::empty({n}, options);
+  // one buffer: slots and positions, then lens and free_count next to each other, cu_new, kv_lens
+  int64_t at_lens = 2 * num_tokens, at_cu = at_lens + n + 1, at_kv = at_cu + n + 1;
+  Tensor all = at::empty({at_kv + n}, tables.options());
+  int* base = all.data_ptr<int>();
   a.tables = tables.data_ptr<int>(), a.lens = lens.data_ptr<int>(), a.new_lens = new_lens.data_ptr<int>();
   a.free_pages = free_pages.data_ptr<int>(), a.free_count = free_count.data_ptr<int>();
-  a.slots = token.data_ptr<int>(), a.positions = a.slots + num_tokens;
-  a.cu_new = cu.data_ptr<int>(), a.kv_lens = kv.data_ptr<int>();
-  a.lens_out = state.data_ptr<int>(), a.free_out = a.lens_out + n;
+  a.slots = base, a.positions = base + num_tokens;
+  a.lens_out = base + at_lens, a.free_out = a.lens_out + n, a.cu_new = base + at_cu, a.kv_lens = base + at_kv;
   a.requests = (int)n, a.width = (int)tables.size(1), a.pages = (int)free_pages.size(0), a.tokens = (int)num_tokens;
   a.table_stride = tables.stride(0);
   launched(paged::launch_plan(a, current_stream()), "plan_step");
-  return {token.select(0, 0), token.select(0, 1), cu, kv, state.narrow(0, 0, n), state.narrow(0, n, 1), state};
+  return {part_of(all, 0, num_tokens), part_of(all, num_tokens, num_tokens), part_of(all, at_cu, n + 1),
+          part_of(all, at_kv, n), part_of(all, at_lens, n), part_of(all, at_lens + n, 1)};
 }
 
 std::vector<Tensor> release_pages(const Tensor& tables, const Tensor& lens, const Tensor& done, const Tensor& free_pages,
@@ -128,7 +137,7 @@ std::vector<Tensor> release_pages(const Tensor& tables, const Tensor& lens, cons
   a.lens_out = state.data_ptr<int>(), a.free_out = a.lens_out + n;
   a.requests = (int)n, a.width = (int)tables.size(1), a.pages = (int)free_pages.size(0), a.table_stride = tables.stride(0);
   launched(paged::launch_release(a, current_stream()), "release_pages");
-  return {state.narrow(0, 0, n), state.narrow(0, n, 1), state};
+  return {part_of(state, 0, n), part_of(state, n, 1)};
 }
 
 void write_kv(const Tensor& k, const Tensor& v, const Tensor& k_cache, const Tensor& v_cache, const Tensor& slots, double k_scale,

@@ -108,8 +108,7 @@ def plan_step(
     once the caller stores them (``PagedKVCache.plan`` does)."""
     ext = _native(tables)
     if ext is not None:
-        got = ext.plan_step(tables, lens, new_lens, free_pages, free_count, page_size, num_tokens)
-        return StepPlan(*got[:6])
+        return StepPlan(*ext.plan_step(tables, lens, new_lens, free_pages, free_count, page_size, num_tokens))
     return _plan_plain(tables, lens, new_lens, free_pages, free_count, page_size, num_tokens)
 
 
@@ -128,8 +127,7 @@ def release_pages(
     pages on the stack twice."""
     ext = _native(tables)
     if ext is not None:
-        got = ext.release_pages(tables, lens, done, free_pages, free_count, page_size)
-        return got[0], got[1]
+        return tuple(ext.release_pages(tables, lens, done, free_pages, free_count, page_size))
     return _release_plain(tables, lens, done, free_pages, free_count, page_size)
 
 
