@@ -85,7 +85,8 @@ bool decode_takes(const AttendArgs& a);
 int64_t decode_workspace(const AttendArgs& a);
 hipError_t launch_decode(const AttendArgs& a, float* workspace, hipStream_t stream);
 bool prompt_takes(const AttendArgs& a);
-hipError_t launch_prompt(const AttendArgs& a, hipStream_t stream);
+int64_t prompt_workspace(const AttendArgs& a);
+hipError_t launch_prompt(const AttendArgs& a, float* workspace, hipStream_t stream);
 hipError_t launch_attend_rows(const AttendArgs& a, hipStream_t stream);
 
 }  // namespace paged

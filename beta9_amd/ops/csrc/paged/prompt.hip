@@ -33,7 +33,13 @@ struct PromptArgs {
   int q_wide;    // q's rows begin on 16 bytes
   int negative;  // the scale is below zero: q's sign is turned instead
   int group, group_log2, kv_heads_log2;  // logarithms: -1 where there is none
+  int target_log2;  // chunks of keys wanted for all tiles of a kv head together; -1: keys are not split
+  float* part;      // [items, kv heads, kRows, dim]: unnormalised sums
+  float* stats;     // [items, kv heads, kRows, 2]: running maximum and sum
 };
+
+// Tiles of keys of a chunk at least.
+constexpr int kLeastTiles = 4;
 
 template <class X> struct Product;
 template <> struct Product<BF16> {
@@ -77,46 +83,84 @@ template <int N> struct Constant {
 
 struct Where {
   int request, tile, row0, rows, keys;  // the request's first packed row, its new tokens and all of them
+  int part, parts, chunk;               // of its keys, the part and its length in tiles of keys
+  int index;                            // where the first of the rows' parts lies in the workspace
 };
 
 // Which rows the item stands for. The tiles that see the most keys come first, so that the last workgroups to start are
 // short ones: up to 64 requests, all tiles are put in order of their last position, in 64 steps (a lane a step counts the
 // tiles in it); among more, the requests follow each other, each from its last tile to its first. On 13 ragged prompts
 // (16 heads of 64, up to 1500 new tokens) 75.8 us, in the requests' order 77.9.
-__device__ inline Where where_of(const AttendArgs& a, int group, int item) {
-  int lane = threadIdx.x & 63, before = 0;
-  for (int first = 0; first < a.requests; first += 64) {
-    int i = first + lane, row0 = 0, n = 0, keys = 0;
+//
+// If there are few tiles, their keys are split: into chunks that are equal for all requests, as for one token. A request's
+// tiles have as many parts as its last one needs; the parts of earlier tiles that hold no keys add nothing. `whole`: the item
+// is a tile with all its parts (for joining them), not one part.
+__device__ inline Where where_of(const PromptArgs& s, int item, bool whole) {
+  const AttendArgs& a = s.a;
+  int lane = threadIdx.x & 63, before = 0, items_before = 0;
+  struct Request {
+    int row0, n, keys, tiles;
+  };
+  auto request = [&](int i) {
+    Request r = {0, 0, 0, 0};
     if (i < a.requests) {
-      row0 = clamp_int(a.cu_new[i], 0, a.rows);
-      n = clamp_int(a.cu_new[i + 1], row0, a.rows) - row0;
-      keys = clamp_int(a.kv_lens[i], 0, a.width << a.page_log2);
+      r.row0 = clamp_int(a.cu_new[i], 0, a.rows);
+      r.n = clamp_int(a.cu_new[i + 1], r.row0, a.rows) - r.row0;
+      r.keys = clamp_int(a.kv_lens[i], 0, a.width << a.page_log2);
     }
-    int tiles = (int)(((int64_t)n * group + kRows - 1) / kRows), from = 0, mine = tiles;
-    if (a.requests > 1 && a.requests <= 64) {
+    r.tiles = (int)(((int64_t)r.n * s.group + kRows - 1) / kRows);
+    return r;
+  };
+  Request mine = request(lane);
+  int chunk = 0;
+  if (s.target_log2 >= 0) {
+    int low = 0, high = 0;
+    for (int i = lane; i < a.requests; i += 64) {
+      Request r = i < 64 ? mine : request(i);
+      int64_t work = (int64_t)r.tiles * ((r.keys + kKeys - 1) / kKeys);
+      low += (int)(work & 0xffff), high += (int)(work >> 16);  // tiles by requests are few here: see kSplitBelow
+    }
+    int64_t total = ((int64_t)whole_sum(high) << 16) + whole_sum(low);
+    chunk = (int)min((int64_t)1 << 30, max((int64_t)kLeastTiles, (total + (1 << s.target_log2) - 1) >> s.target_log2));
+  }
+  for (int first = 0; first < a.requests; first += 64) {
+    Request r = first ? request(first + lane) : mine;
+    int from = 0, count = r.tiles, parts = 1;
+    if (chunk) {
+      parts = max(1, ((r.keys + kKeys - 1) / kKeys + chunk - 1) / chunk);
+      count = whole ? r.tiles : r.tiles * parts;
+    } else if (a.requests > 1 && a.requests <= 64) {
       // in tiles' places: the request's begin behind what it held before
-      int start = (int)(min((int64_t)max(keys - n, 0) * group, (int64_t)1 << 30) / kRows), end = start + tiles;
-      int width = (whole_max(end) + 63) / 64, low = (63 - lane) * width, count = 0;
-      for (int r = 0; r < a.requests; r++)
-        count += clamp_int(lane_value(end, r) - low, 0, width) - clamp_int(lane_value(start, r) - low, 0, width);
-      int up = running_sum(count);
+      int start = (int)(min((int64_t)max(r.keys - r.n, 0) * s.group, (int64_t)1 << 30) / kRows), end = start + r.tiles;
+      int width = (whole_max(end) + 63) / 64, low = (63 - lane) * width, here = 0;
+      for (int i = 0; i < a.requests; i++)
+        here += clamp_int(lane_value(end, i) - low, 0, width) - clamp_int(lane_value(start, i) - low, 0, width);
+      int up = running_sum(here);
       uint64_t found = __ballot(up > item);
       if (!found) break;
       int at = __builtin_ctzll(found);
-      item -= lane_value(up, at) - lane_value(count, at);
+      item -= lane_value(up, at) - lane_value(here, at);
       low = (63 - at) * width;
-      from = clamp_int(low - start, 0, tiles);
-      mine = clamp_int(low + width - start, 0, tiles) - from;
+      from = clamp_int(low - start, 0, r.tiles);
+      count = clamp_int(low + width - start, 0, r.tiles) - from;
     }
-    int up = running_sum(mine);
+    int up = running_sum(count), items_up = chunk ? running_sum(r.tiles * parts) : 0;
     uint64_t found = __ballot(before + up > item);
     if (found) {
-      int at = __builtin_ctzll(found);
-      return {first + at, lane_value(from, at) + before + lane_value(up, at) - 1 - item, lane_value(row0, at), lane_value(n, at), lane_value(keys, at)};
+      int at = __builtin_ctzll(found), local = item - before - lane_value(up - count, at);
+      Where w = {first + at, 0, lane_value(r.row0, at), lane_value(r.n, at), lane_value(r.keys, at), 0, lane_value(parts, at), chunk, 0};
+      int back = chunk && !whole ? local / w.parts : local;  // tiles from the last
+      w.tile = lane_value(from + count, at) - 1 - back;
+      if (chunk) {
+        w.tile = lane_value(r.tiles, at) - 1 - back;
+        w.part = whole ? 0 : local - back * w.parts;
+        w.index = items_before + lane_value(items_up - r.tiles * parts, at) + back * w.parts;
+      }
+      return w;
     }
-    before += lane_value(up, 63);
+    before += lane_value(up, 63), items_before += lane_value(items_up, 63);
   }
-  return {-1, 0, 0, 0, 0};
+  return {-1, 0, 0, 0, 0, 0, 1, 0, 0};
 }
 
 template <class X, class C, int D>
@@ -142,7 +186,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : 2) void prompt_kernel(Pr
       for (int i = tid; i < a.heads * D; i += kWaves * 64) out[(i / D) * a.out_head + i % D] = (Out)0.f;
     }
   };
-  Where w = where_of(a, s.group, item);
+  Where w = where_of(s, item, false);
   if (w.request < 0) {
     clear_rest();
     return;
@@ -159,7 +203,8 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : 2) void prompt_kernel(Pr
   int position = ahead + token;
   int low = ahead + by_group(min(wave_first, packed - 1)), high = ahead + by_group(min(wave_first + 31, packed - 1));
   int last = ahead + by_group(min(row_first + kRows - 1, packed - 1));  // the workgroup's last position
-  int tiles = last < 0 ? 0 : min(last, length - 1) / kKeys + 1;
+  int begin = w.part * w.chunk, end = last < 0 ? 0 : min(last, length - 1) / kKeys + 1;  // tiles of keys
+  if (w.parts > 1) end = min(end, begin + w.chunk);
 
   const int* table = a.tables + w.request * a.table_stride;
   const char* caches[2] = {(const char*)a.k_cache, (const char*)a.v_cache};
@@ -327,6 +372,12 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : 2) void prompt_kernel(Pr
   };
   auto present_of = [&](int entry) { return __ballot((unsigned)entry < (unsigned)a.pages); };
 
+  // The last loads into LDS, which nobody reads, are there before it is used for something else or given back.
+  auto finish = [&]() {
+    if constexpr (!kNarrow) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  };
+
   // One pass over the keys. A tile's scores are made in the step before its own, so that the matrix instructions of the
   // next tile's scores and the exponentials of this one's fill each other's gaps within a wave; K is therefore a tile
   // ahead of V. A later token's value that is not finite would reach the rows that do not see it through 0 * inf;
@@ -335,16 +386,16 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : 2) void prompt_kernel(Pr
 #pragma unroll
     for (int d = 0; d < kDims; d++) acc[d] = f32x16{};
     m = kMinusInf, l = 0.f;
-    if (!tiles) return;
-    int mine = high < 0 ? 0 : min(tiles, high / kKeys + 1);  // the wave's own tiles
+    if (begin >= end) return;
+    int mine = high < 0 ? 0 : min(end, high / kKeys + 1);  // where the wave's own tiles end
     if constexpr (!kAhead) {
-      int entry0 = entry_of(0), entry1 = entry_of(1);
+      int entry0 = entry_of(begin), entry1 = entry_of(begin + 1);
       if constexpr (kNarrow) {
-        fetch(0, 0, entry0), put(0, 0);
-        fetch(1, 0, entry0), put(1, 0);
+        fetch(0, begin, entry0), put(0, 0);
+        fetch(1, begin, entry0), put(1, 0);
       } else {
-        stage(0, 0, 0, entry0);
-        stage(1, 0, 0, entry0);
+        stage(0, begin, 0, entry0);
+        stage(1, begin, 0, entry0);
       }
       if (!careful) load_q();
       auto step = [&](auto which, int tile) {
@@ -381,22 +432,22 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : 2) void prompt_kernel(Pr
         if constexpr (kNarrow) put(1, buffer ^ 1);
         entry0 = entry1, entry1 = entry2;
       };
-      for (int tile = 0; tile < tiles; tile += 2) {
+      for (int tile = begin; tile < end; tile += 2) {
         step(Constant<0>{}, tile);
-        if (tile + 1 < tiles) step(Constant<1>{}, tile + 1);
+        if (tile + 1 < end) step(Constant<1>{}, tile + 1);
       }
-      __syncthreads();
+      finish();
       return;
     } else {
-    int entry0 = entry_of(0), entry1 = entry_of(1), entry2 = entry_of(2);  // of this tile and the next two
+    int entry0 = entry_of(begin), entry1 = entry_of(begin + 1), entry2 = entry_of(begin + 2);  // of this tile and the next two
     if constexpr (kNarrow) {
-      fetch(0, 0, entry0), put(0, 0);
-      fetch(1, 0, entry0), put(1, 0);
-      fetch(0, 1, entry1), put(0, 1);
+      fetch(0, begin, entry0), put(0, 0);
+      fetch(1, begin, entry0), put(1, 0);
+      fetch(0, begin + 1, entry1), put(0, 1);
     } else {
-      stage(0, 0, 0, entry0);
-      stage(1, 0, 0, entry0);
-      stage(0, 1, 1, entry1);
+      stage(0, begin, 0, entry0);
+      stage(1, begin, 0, entry0);
+      stage(0, begin + 1, 1, entry1);
     }
     if (!careful) load_q();
     if constexpr (!kNarrow) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -404,7 +455,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : 2) void prompt_kernel(Pr
     f32x16 x[2];
     scores(0, x);
     uint64_t present = present_of(entry0);
-    bool whole = mask(x, 0, present);
+    bool whole = mask(x, begin * kKeys, present);
     raise(highest(x));
     // one step: x holds the tile's scores, y takes the next's
     auto step = [&](auto which, int tile, f32x16 (&x)[2], f32x16 (&y)[2]) {
@@ -461,11 +512,11 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : 2) void prompt_kernel(Pr
       entry1 = entry2, entry2 = entry3;
     };
     f32x16 y[2];
-    for (int tile = 0; tile < tiles; tile += 2) {
+    for (int tile = begin; tile < end; tile += 2) {
       step(Constant<0>{}, tile, x, y);
-      if (tile + 1 < tiles) step(Constant<1>{}, tile + 1, y, x);
+      if (tile + 1 < end) step(Constant<1>{}, tile + 1, y, x);
     }
-    __syncthreads();
+    finish();
     }
   };
   pass(Constant<0>{});
@@ -484,6 +535,16 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : 2) void prompt_kernel(Pr
 
   clear_rest();
   l += __shfl_xor(l, 32);
+  if (w.parts > 1) {
+    int64_t at = ((int64_t)(w.index + w.part) * a.kv_heads + kv_head) * kRows + wave * 32 + n;
+    if (half == 0) *reinterpret_cast<f32x2*>(s.stats + 2 * at) = f32x2{m, l};
+#pragma unroll
+    for (int d = 0; d < kDims; d++)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4)
+        *reinterpret_cast<f32x4*>(s.part + at * D + 4 * half + 32 * d + 2 * r) = f32x4{acc[d][r], acc[d][r + 1], acc[d][r + 2], acc[d][r + 3]};
+    return;
+  }
   float f = l == 0.f ? 0.f : a.value_scale / l;
   if (!real) return;
   Out* out = (Out*)a.out + (w.row0 + token) * a.out_row + head * a.out_head + 4 * half;
@@ -498,11 +559,67 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : 2) void prompt_kernel(Pr
     }
 }
 
+// Joins the parts of some rows of a tile and a kv head: D / 4 threads a row, eight parts on their way at a time.
+template <class X, int D>
+__global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs s) {
+  const AttendArgs& a = s.a;
+  int item = blockIdx.x / a.kv_heads, kv_head = blockIdx.x - item * a.kv_heads;
+  Where w = where_of(s, item, true);
+  if (w.request < 0 || w.parts <= 1) return;
+  constexpr int kLanes = D / 4, kAhead = 8;
+  int dim = (threadIdx.x % kLanes) * 4, r = blockIdx.y * (256 / kLanes) + threadIdx.x / kLanes, row = w.tile * kRows + r;
+  if (row >= w.rows * s.group) return;
+  float m = kMinusInf, l = 0.f;
+  f32x4 o = {};
+  for (int i = 0; i < w.parts; i += kAhead) {
+    f32x4 x[kAhead];
+    f32x2 stat[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; j++) {
+      int64_t at = ((int64_t)(w.index + min(i + j, w.parts - 1)) * a.kv_heads + kv_head) * kRows + r;
+      x[j] = *reinterpret_cast<const f32x4*>(s.part + at * D + dim);
+      stat[j] = *reinterpret_cast<const f32x2*>(s.stats + 2 * at);
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; j++) {
+      if (i + j >= w.parts || stat[j][0] == kMinusInf) continue;  // no key of the part is seen
+      float top = fmaxf(m, stat[j][0]), f = __builtin_amdgcn_exp2f(m - top), g = __builtin_amdgcn_exp2f(stat[j][0] - top);
+      l = f * l + g * stat[j][1], o = f * o + g * x[j];
+      m = top;
+    }
+  }
+  int token = row / s.group, head = kv_head * s.group + row - token * s.group;
+  typename X::T* out = (typename X::T*)a.out + (w.row0 + token) * a.out_row + head * a.out_head + dim;
+  float f = l == 0.f ? 0.f : a.value_scale / l;
+  typename Vec<X>::x4 y;
+#pragma unroll
+  for (int i = 0; i < 4; i++) y[i] = (typename X::T)(l == 0.f ? 0.f : o[i] * f);
+  *reinterpret_cast<typename Vec<X>::x4*>(out) = y;
+}
+
+int64_t tiles_of(const AttendArgs& a) { return ((int64_t)a.rows * (a.heads / a.kv_heads)) / kRows + a.requests; }
+
+// Where fewer workgroups than this would start, and a row may see more keys than four chunks, the keys are split over about
+// as many. 16 tokens behind 4096 (32 heads over 8 of 128) take 18.3 us, 70.4 without; over twice as many parts 18.7, and one
+// token behind 16000 34 us instead of 26, for the joining. Among 256 tokens with nothing before them it would not pay.
+constexpr int kSplitBelow = 256;
+int split_log2_of(const AttendArgs& a) {
+  if (tiles_of(a) * a.kv_heads >= kSplitBelow || ((int64_t)a.width << a.page_log2) <= 4 * kLeastTiles * kKeys) return -1;
+  int log2 = 0;
+  while ((2LL << log2) * a.kv_heads <= kSplitBelow) log2++;
+  return log2;
+}
+
 }  // namespace
 
 bool prompt_takes(const AttendArgs& a) { return a.dim == 64 || a.dim == 128; }
 
-hipError_t launch_prompt(const AttendArgs& a, hipStream_t stream) {
+int64_t prompt_workspace(const AttendArgs& a) {
+  int log2 = split_log2_of(a);
+  return log2 < 0 ? 0 : (tiles_of(a) + (1LL << log2)) * a.kv_heads * kRows * (a.dim + 2);
+}
+
+hipError_t launch_prompt(const AttendArgs& a, float* workspace, hipStream_t stream) {
   PromptArgs s;
   s.a = a;
   s.q_wide = (uintptr_t)a.q % 16 == 0 && (a.q_row | a.q_head) % 8 == 0;
@@ -511,13 +628,20 @@ hipError_t launch_prompt(const AttendArgs& a, hipStream_t stream) {
   s.a.score_scale = a.score_scale == 0 ? 0x1p-100f : (s.negative ? -a.score_scale : a.score_scale);
   auto log2 = [](int x) { return x & (x - 1) ? -1 : __builtin_ctz(x); };
   s.group = a.heads / a.kv_heads, s.group_log2 = log2(s.group), s.kv_heads_log2 = log2(a.kv_heads);
-  int64_t items = ((int64_t)a.rows * s.group) / kRows + a.requests;
+  int64_t tiles = tiles_of(a), items = tiles;
   if (items < 1) items = 1;
+  s.target_log2 = split_log2_of(a);
+  if (s.target_log2 >= 0) items += 1LL << s.target_log2;
+  s.part = workspace, s.stats = workspace + items * a.kv_heads * kRows * a.dim;
   if (items * a.kv_heads >= (1LL << 31)) return hipErrorInvalidValue;
   dim3 grid((unsigned)(items * a.kv_heads));
 #define LAUNCH(X, C) (a.dim == 64 ? launch(prompt_kernel<X, C, 64>, grid, kWaves * 64, stream, s) : launch(prompt_kernel<X, C, 128>, grid, kWaves * 64, stream, s))
-  return PAGED_DISPATCH(a.type, a.cache, LAUNCH);
+  hipError_t status = PAGED_DISPATCH(a.type, a.cache, LAUNCH);
 #undef LAUNCH
+  if (status != hipSuccess || s.target_log2 < 0 || !tiles) return status;
+  dim3 joins((unsigned)(tiles * a.kv_heads), kRows / (256 / (a.dim / 4)));
+  if (a.type == Type::kBF16) return a.dim == 64 ? launch(prompt_join_kernel<BF16, 64>, joins, 256, stream, s) : launch(prompt_join_kernel<BF16, 128>, joins, 256, stream, s);
+  return a.dim == 64 ? launch(prompt_join_kernel<FP16, 64>, joins, 256, stream, s) : launch(prompt_join_kernel<FP16, 128>, joins, 256, stream, s);
 }
 
 }  // namespace paged

@@ -354,6 +354,47 @@ def test_prompt_attention_over_many_tiles(device, kind, cached, dim, page):
 
 
 @both
+@pytest.mark.parametrize("kind,cached", KINDS)
+@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 4, 4), (128, 8, 2), (128, 5, 1), (64, 40, 1)])
+@pytest.mark.parametrize(
+    "new,held",
+    [([7], [3000]), ([1, 0, 40, 3], [2500, 900, 0, 1023]), ([130], [1100]), ([2] * 70, [600 + 13 * i for i in range(70)])],
+)
+def test_prompt_attention_of_few_rows_over_many_keys(device, kind, cached, dim, heads, kv_heads, new, held):
+    """The last tokens of a request behind a long beginning, one, several and more than 64 requests."""
+    if len(new) > 4 and (heads, kind, cached) != (8, "bf16", "bf16"):
+        pytest.skip("once is enough")
+    gen = torch.Generator().manual_seed(len(new) + dim)
+    lens = [h + n for h, n in zip(held, new)]
+    cu = [0]
+    for n in new:
+        cu.append(cu[-1] + n)
+    cache = make_cache(gen, lens, kv_heads, dim, 32, kind, cached, device)
+    q = (torch.randn((cu[-1] + 3, heads, dim), generator=gen) * 2).to(TYPES[kind]).to(device)
+    got = run_prompt(q, cache, lens, cu)
+    assert (got[cu[-1] :] == 0).all()
+    check_attention(got[: cu[-1]], q[: cu[-1]], cache, lens, cu)
+
+
+@both
+@pytest.mark.parametrize("dim", [64, 128])
+def test_split_keys_with_bad_entries_and_values(device, dim):
+    """The same with an entry that names no page, and a later token that is not finite, in different parts of the keys."""
+    gen = torch.Generator().manual_seed(dim)
+    k_cache, v_cache, tables, scales = make_cache(gen, [2100], 2, dim, 16, "bf16", "bf16", device)
+    cache = (k_cache, v_cache, tables, scales)
+    q = torch.randn((60, 4, dim), generator=gen).to(torch.bfloat16).to(device)
+    tables[0][20], tables[0][100] = -1, 1 << 30
+    clean = run_prompt(q, cache, [2100], [0, 60])
+    check_attention(clean, q, cache, [2100], [0, 60])
+    v_cache[tables[0][2090 // 16], 0, 2090 % 16, 3] = math.nan
+    got = run_prompt(q, cache, [2100], [0, 60])
+    check_attention(got[:50], q[:50], cache, [2090], [0, 50])
+    check_attention(got[:, 2:], q[:, 2:], (k_cache[:, 1:], v_cache[:, 1:], tables, scales), [2100], [0, 60])
+    assert got[50:, :2, 3].isnan().all() and got[50:, :2, 4:].isfinite().all()
+
+
+@both
 @pytest.mark.parametrize("dim", [80, 64, 128])
 def test_attention_with_entries_that_name_no_page(device, dim):
     """Their tokens count as absent, whatever the other pages hold."""
