@@ -178,9 +178,10 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : 2) void prompt_kernel(Pr
   int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5, n = lane & 31;
   int item = s.kv_heads_log2 >= 0 ? blockIdx.x >> s.kv_heads_log2 : blockIdx.x / a.kv_heads, kv_head = blockIdx.x - item * a.kv_heads;
 
+  int rest = a.cu_new[a.requests], front = a.cu_new[0];  // on their way while the rest goes on
   auto clear_rest = [&]() {
     if (!a.clear_rest) return;
-    int rest = clamp_int(a.cu_new[a.requests], 0, a.rows), front = clamp_int(a.cu_new[0], 0, a.rows);
+    rest = clamp_int(rest, 0, a.rows), front = clamp_int(front, 0, a.rows);
     for (int64_t r = blockIdx.x; r < front + (int64_t)a.rows - rest; r += gridDim.x) {
       Out* out = (Out*)a.out + (r < front ? r : r - front + rest) * a.out_row;
       for (int i = tid; i < a.heads * D; i += kWaves * 64) out[(i / D) * a.out_head + i % D] = (Out)0.f;
@@ -546,8 +547,9 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : 2) void prompt_kernel(Pr
     return;
   }
   float f = l == 0.f ? 0.f : a.value_scale / l;
-  if (!real) return;
-  Out* out = (Out*)a.out + (w.row0 + token) * a.out_row + head * a.out_head + 4 * half;
+  // Through the wave's part of LDS, so that each store fills whole lines: with 16 bytes of 32 rows a store, the results of a
+  // workgroup (head dim 128) took 2 us and more. Chunks are exchanged by the row as for K.
+  char* mine = lds + wave * 32 * kRowBytes;
 #pragma unroll
   for (int d = 0; d < kDims; d++)
 #pragma unroll
@@ -555,8 +557,16 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : 2) void prompt_kernel(Pr
       typename Vec<X>::x4 y;
 #pragma unroll
       for (int i = 0; i < 4; i++) y[i] = (Out)(l == 0.f ? 0.f : acc[d][r + i] * f);
-      *reinterpret_cast<typename Vec<X>::x4*>(out + 32 * d + 2 * r) = y;
+      *reinterpret_cast<typename Vec<X>::x4*>(mine + n * kRowBytes + (((4 * d + r / 4) ^ (n & (kChunks - 1))) * 16) + 8 * half) = y;
     }
+  int place = real ? (w.row0 + token) * a.heads + head : -1;  // fits: rows by heads do; `out` has no gaps
+#pragma unroll
+  for (int i = 0; i < 32 * kChunks / 64; i++) {
+    int from = i * (64 / kChunks) + lane / kChunks, chunk = lane % kChunks;
+    int to = __shfl(place, from);
+    u32x4 y = *reinterpret_cast<const u32x4*>(mine + from * kRowBytes + chunk * 16);
+    if (to >= 0) *reinterpret_cast<u32x4*>((Out*)a.out + (int64_t)to * D + (chunk ^ (from & (kChunks - 1))) * 8) = y;
+  }
 }
 
 // Joins the parts of some rows of a tile and a kv head: D / 4 threads a row, eight parts on their way at a time.
