@@ -216,17 +216,12 @@ Tensor attend(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, con
   a.width = (int)tables.size(1), a.pages = (int)k_cache.size(0);
   a.score_scale = (float)(scale * k_scale * kLog2E), a.value_scale = (float)v_scale;
   a.clear_rest = out_given ? 0 : 1;
-  bool fast = cu_new ? paged::prompt_takes(a) : paged::decode_takes(a);
-  if (fast) {
-    int64_t floats = cu_new ? paged::prompt_workspace(a) : paged::decode_workspace(a);
-    Tensor workspace;
-    if (floats) workspace = at::empty({floats}, q.options().dtype(at::kFloat));
-    float* space = floats ? workspace.data_ptr<float>() : nullptr;
-    launched(cu_new ? paged::launch_prompt(a, space, current_stream()) : paged::launch_decode(a, space, current_stream()),
-             cu_new ? "prompt_attention" : "decode_attention");
-    return out;
-  }
-  launched(paged::launch_attend_rows(a, current_stream()), cu_new ? "prompt_attention" : "decode_attention");
+  int64_t floats = cu_new ? paged::prompt_workspace(a) : paged::decode_workspace(a);
+  Tensor workspace;
+  if (floats) workspace = at::empty({floats}, q.options().dtype(at::kFloat));
+  float* space = floats ? workspace.data_ptr<float>() : nullptr;
+  launched(cu_new ? paged::launch_prompt(a, space, current_stream()) : paged::launch_decode(a, space, current_stream()),
+           cu_new ? "prompt_attention" : "decode_attention");
   return out;
 }
 

@@ -75,11 +75,13 @@ __device__ inline Share share_of(const SplitArgs& s, int item, int request_wante
   return {-1, 0, 0, 0, 0};
 }
 
-template <class X, class C, int D> struct Decode {
+// D: 64, 128 or 256. A smaller head dim takes the next of these (kPad): what lies past it is zero in the registers.
+template <class X, class C, int D, bool kPad> struct Decode {
   static constexpr int kPer = D / 16;                       // dims of V a lane loads
   static constexpr bool kNarrow = sizeof(typename C::T) == 1;
+  static constexpr int kSize = kNarrow ? 1 : 2;
   static constexpr int kLoads = kNarrow ? D / 64 : D / 32;  // 16-byte loads of a row of K a lane makes
-  static constexpr int kVWords = kPer * (int)sizeof(typename C::T) / 4;
+  static constexpr int kVBytes = kPer * kSize, kVLoads = kVBytes > 16 ? kVBytes / 16 : 1, kVWords = kVBytes / kVLoads / 4;
   // The exponent's offset and how far a score may pass the running maximum before the sums are rescaled. fp16 holds
   // probabilities down to 2^-24: 2^8 times larger, what is lost is below 2^-32 of the largest.
   static constexpr float kBias = __is_same(X, FP16) ? 8.f : 0.f;
@@ -88,7 +90,7 @@ template <class X, class C, int D> struct Decode {
 
   struct Tile {
     u32x4 k[2][kLoads];
-    Words<kVWords> v[8];
+    Words<kVWords> v[8][kVLoads];
     bool known;  // this lane's keys 8g .. 8g + 7 lie on a page
   };
 
@@ -105,6 +107,23 @@ template <class X, class C, int D> struct Decode {
       return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, kHigh));
     else
       return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, kHigh));
+  }
+
+  // kBytes from `row` + `at` bytes, as far as the row's `size` goes (a multiple of 8; words of 4 bytes: of 4)
+  template <int kWords> static __device__ Words<kWords> part(const char* row, int at, int size) {
+    if constexpr (!kPad) return *reinterpret_cast<const Words<kWords>*>(row + at);
+    Words<kWords> x = Words<kWords>(0);
+    if constexpr (kWords == 4) {
+      if (at + 16 <= size) {
+        x = *reinterpret_cast<const Words<4>*>(row + at);
+      } else if (at + 8 <= size) {
+        u32x2 y = *reinterpret_cast<const u32x2*>(row + at);
+        x[0] = y[0], x[1] = y[1];
+      }
+    } else {
+      if (at + 4 * kWords <= size) x = *reinterpret_cast<const Words<kWords>*>(row + at);
+    }
+    return x;
   }
 
   // the operand of k-step s of a row of K
@@ -125,9 +144,9 @@ template <class X, class C, int D> struct Decode {
   static __device__ int k_dim(int s, int g) { return kNarrow ? (s >> 1) * 64 + g * 16 + (s & 1) * 8 : s * 32 + g * 8; }
 };
 
-template <class X, class C, int D>
-__global__ __launch_bounds__(kWaves * 64, 4) void split_kernel(SplitArgs s) {
-  typedef Decode<X, C, D> K;
+template <class X, class C, int D, bool kPad>
+__global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : 4) void split_kernel(SplitArgs s) {
+  typedef Decode<X, C, D, kPad> K;
   typedef typename K::Half8 Half8;
   const AttendArgs& a = s.a;
   __shared__ float o_lds[kWaves][kHeads][D + 4];
@@ -148,7 +167,7 @@ __global__ __launch_bounds__(kWaves * 64, 4) void split_kernel(SplitArgs s) {
     for (int i = 0; i < D / 32; i++) {
       const typename X::T* p = row + K::k_dim(i, g);
       Half8 x = {};
-      if (c < heads_here) {
+      if (c < heads_here && (!kPad || K::k_dim(i, g) < a.dim)) {
         if (s.q_wide) {
           x = *reinterpret_cast<const Half8*>(p);
         } else {
@@ -161,27 +180,30 @@ __global__ __launch_bounds__(kWaves * 64, 4) void split_kernel(SplitArgs s) {
   }
 
   const int* table = a.tables + share.request * a.table_stride;
-  const typename C::T* k_cache = (const typename C::T*)a.k_cache;
-  const typename C::T* v_cache = (const typename C::T*)a.v_cache;
+  const char* k_cache = (const char*)a.k_cache;
+  const char* v_cache = (const char*)a.v_cache;
+  int row_bytes = (kPad ? a.dim : D) * K::kSize;
   int in_page = (1 << a.page_log2) - 1;
   // this lane's 8 keys: of K by its row, of V by its place; both lie on one page each
   auto entry_of = [&](int key) { return table[min(key >> a.page_log2, a.width - 1)]; };
   auto offset_of = [&](int page, int key) {
-    return ((((int64_t)page * a.kv_heads + kv_head) << a.page_log2) + (key & in_page)) * D;
+    return ((((int64_t)page * a.kv_heads + kv_head) << a.page_log2) + (key & in_page)) * row_bytes;
   };
   int k_key = 8 * (c >> 2) + (c & 3), v_key = 8 * g;
   auto fetch = [&](typename K::Tile& t, int base, int k_page, int v_page) {
     bool k_known = (unsigned)k_page < (unsigned)a.pages;
     t.known = (unsigned)v_page < (unsigned)a.pages;
-    const typename C::T* k = k_cache + offset_of(k_known ? k_page : 0, base + k_key);
-    const typename C::T* v = v_cache + offset_of(t.known ? v_page : 0, base + v_key) + c * K::kPer;
+    const char* k = k_cache + offset_of(k_known ? k_page : 0, base + k_key);
+    const char* v = v_cache + offset_of(t.known ? v_page : 0, base + v_key);
 #pragma unroll
     for (int h = 0; h < 2; h++)
 #pragma unroll
-      for (int i = 0; i < K::kLoads; i++)
-        t.k[h][i] = *reinterpret_cast<const u32x4*>(k + 4 * h * D + (i * 4 + g) * (16 / (int)sizeof(typename C::T)));
+      for (int i = 0; i < K::kLoads; i++) t.k[h][i] = K::template part<4>(k + 4 * h * row_bytes, (i * 4 + g) * 16, row_bytes);
 #pragma unroll
-    for (int j = 0; j < 8; j++) t.v[j] = *reinterpret_cast<const Words<K::kVWords>*>(v + j * D);
+    for (int j = 0; j < 8; j++)
+#pragma unroll
+      for (int i = 0; i < K::kVLoads; i++)
+        t.v[j][i] = K::template part<K::kVWords>(v + j * row_bytes, c * K::kVBytes + i * 16, row_bytes);
   };
 
   f32x4 acc[K::kPer] = {};
@@ -201,7 +223,9 @@ __global__ __launch_bounds__(kWaves * 64, 4) void split_kernel(SplitArgs s) {
 #pragma unroll
       for (int j = 0; j < 8; j++) {
         x[j] = j < here ? x[j] : kMinusInf;
-        if (j >= here) t.v[j] = Words<K::kVWords>(0);  // what lies there may be no number
+#pragma unroll
+        for (int i = 0; i < K::kVLoads; i++)
+          if (j >= here) t.v[j][i] = Words<K::kVWords>(0);  // what lies there may be no number
       }
     }
 #pragma unroll
@@ -232,10 +256,13 @@ __global__ __launch_bounds__(kWaves * 64, 4) void split_kernel(SplitArgs s) {
     for (int j = 0; j < 8; j++)
 #pragma unroll
       for (int i = 0; i < K::kPer / 2; i++) {
-        if constexpr (K::kNarrow)
-          w[j][i] = i & 1 ? K::template widen<true>(t.v[j][i >> 1]) : K::template widen<false>(t.v[j][i >> 1]);
-        else
-          w[j][i] = t.v[j][i];
+        constexpr int kEach = K::kVWords;
+        if constexpr (K::kNarrow) {
+          uint32_t x = t.v[j][(i >> 1) / kEach][(i >> 1) % kEach];
+          w[j][i] = i & 1 ? K::template widen<true>(x) : K::template widen<false>(x);
+        } else {
+          w[j][i] = t.v[j][i / kEach][i % kEach];
+        }
       }
     // An infinite value makes its sums infinite; a second part of zero or of another sign would make them NaN. (e4m3 has
     // no infinities.)
@@ -300,7 +327,8 @@ __global__ __launch_bounds__(kWaves * 64, 4) void split_kernel(SplitArgs s) {
     typename X::T* out = (typename X::T*)a.out + share.request * a.out_row + (head0 + head) * a.out_head + dim;
     float f = sum == 0.f ? 0.f : a.value_scale / sum;
 #pragma unroll
-    for (int i = 0; i < K::kPer; i++) out[i] = (typename X::T)(sum == 0.f ? 0.f : o[i] * f);
+    for (int i = 0; i < K::kPer; i++)
+      if (!kPad || dim + i < a.dim) out[i] = (typename X::T)(sum == 0.f ? 0.f : o[i] * f);
   } else {
     int64_t at = (int64_t)blockIdx.x * a.heads + head0 + head;
 #pragma unroll
@@ -350,7 +378,7 @@ __global__ __launch_bounds__(kWaves * 64) void join_kernel(SplitArgs s) {
   *reinterpret_cast<f32x4*>(&o_lds[slot][here][dim]) = o;
   if (dim == 0) m_lds[slot][here] = m, l_lds[slot][here] = l;
   __syncthreads();
-  if (slot || !real) return;
+  if (slot || !real || dim >= a.dim) return;
   float top = m;
 #pragma unroll
   for (int w = 1; w < kSlots; w++) top = fmaxf(top, m_lds[w][here]);
@@ -397,10 +425,8 @@ int64_t items_of(const AttendArgs& a) {
 }  // namespace
 
 int64_t decode_workspace(const AttendArgs& a) {
-  return target_log2_of(a) < 0 ? 0 : items_of(a) * a.heads * (a.dim + 2);
+  return target_log2_of(a) < 0 ? 0 : items_of(a) * a.heads * (padded_dim(a.dim) + 2);
 }
-
-bool decode_takes(const AttendArgs& a) { return a.dim == 64 || a.dim == 128; }
 
 hipError_t launch_decode(const AttendArgs& a, float* workspace, hipStream_t stream) {
   SplitArgs s;
@@ -410,19 +436,21 @@ hipError_t launch_decode(const AttendArgs& a, float* workspace, hipStream_t stre
   // not split: chunks of kOne, whatever the sum of the lengths is
   s.target_log2 = split ? log2 : 30, s.least = split ? kLeast : kOne;
   int64_t items = items_of(a);
-  s.part = workspace, s.stats = workspace + items * a.heads * a.dim;
+  s.part = workspace, s.stats = workspace + items * a.heads * padded_dim(a.dim);
   s.q_wide = (uintptr_t)a.q % 16 == 0 && (a.q_row | a.q_head) % 8 == 0;
   dim3 grid((unsigned)items, (unsigned)columns_of(a));
-#define LAUNCH(X, C) (a.dim == 64 ? launch(split_kernel<X, C, 64>, grid, kWaves * 64, stream, s) : launch(split_kernel<X, C, 128>, grid, kWaves * 64, stream, s))
+#define LAUNCH_DIM(X, C, D) (a.dim == D ? launch(split_kernel<X, C, D, false>, grid, kWaves * 64, stream, s) : launch(split_kernel<X, C, D, true>, grid, kWaves * 64, stream, s))
+#define LAUNCH(X, C) PAGED_DIM(a.dim, LAUNCH_DIM, X, C)
   hipError_t status = PAGED_DISPATCH(a.type, a.cache, LAUNCH);
 #undef LAUNCH
+#undef LAUNCH_DIM
   if (status != hipSuccess || !split) return status;
   bool few = (int64_t)a.requests * a.heads <= kFewRows;
-  dim3 rows((unsigned)a.requests, (unsigned)(few ? a.heads : (a.heads + 7) / 8));
-#define LAUNCH(X, D) (few ? launch(join_kernel<X, D, 1>, rows, kWaves * 64, stream, s) : launch(join_kernel<X, D, 8>, rows, kWaves * 64, stream, s))
-  if (a.type == Type::kBF16) return a.dim == 64 ? LAUNCH(BF16, 64) : LAUNCH(BF16, 128);
-  return a.dim == 64 ? LAUNCH(FP16, 64) : LAUNCH(FP16, 128);
-#undef LAUNCH
+  int join = few ? 1 : (a.dim > 128 ? 4 : 8);
+  dim3 rows((unsigned)a.requests, (unsigned)((a.heads + join - 1) / join));
+#define LAUNCH_DIM(X, C, D) (few ? launch(join_kernel<X, D, 1>, rows, kWaves * 64, stream, s) : launch(join_kernel<X, D, D == 256 ? 4 : 8>, rows, kWaves * 64, stream, s))
+  return a.type == Type::kBF16 ? PAGED_DIM(a.dim, LAUNCH_DIM, BF16, BF16) : PAGED_DIM(a.dim, LAUNCH_DIM, FP16, FP16);
+#undef LAUNCH_DIM
 }
 
 }  // namespace paged

@@ -30,37 +30,6 @@ template <class C> struct Vec {
 
 constexpr float kMinusInf = -__builtin_inff();
 
-template <class C> __device__ inline float to_float(typename C::T x) { return (float)x; }
-template <> __device__ inline float to_float<E4M3>(uint8_t x) {
-  return __builtin_amdgcn_cvt_f32_fp8(x, 0);
-}
-
-// 8 neighbours of 16 bytes (8 bytes of e4m3) in 32 bits.
-template <class C> __device__ inline void load8(const typename C::T* p, float (&x)[8]) {
-  typename Vec<C>::x8 v = *reinterpret_cast<const typename Vec<C>::x8*>(p);
-#pragma unroll
-  for (int i = 0; i < 8; i++) x[i] = (float)v[i];
-}
-template <> __device__ inline void load8<E4M3>(const uint8_t* p, float (&x)[8]) {
-  u32x2 v = *reinterpret_cast<const u32x2*>(p);
-#pragma unroll
-  for (int i = 0; i < 2; i++) {
-    f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(v[i], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(v[i], true);
-    x[4 * i] = lo[0], x[4 * i + 1] = lo[1], x[4 * i + 2] = hi[0], x[4 * i + 3] = hi[1];
-  }
-}
-
-__device__ inline float wave_max(float x) {
-#pragma unroll
-  for (int m = 32; m; m >>= 1) x = fmaxf(x, __shfl_xor(x, m));
-  return x;
-}
-__device__ inline float wave_sum(float x) {
-#pragma unroll
-  for (int m = 32; m; m >>= 1) x += __shfl_xor(x, m);
-  return x;
-}
-
 // Inclusive sums, the sum and the maximum over the lanes of whole numbers, by moves within the registers: about 50 cycles,
 // where exchanges through LDS take 130 for each of the six steps.
 template <int kControl, int kRows> __device__ inline int moved(int x, int otherwise) {
@@ -113,5 +82,9 @@ template <class Args> inline hipError_t launch(void (*kernel)(Args), dim3 grid, 
 #define PAGED_DISPATCH(type, cache, F)                                                      \
   ((cache) == Type::kE4M3 ? ((type) == Type::kBF16 ? F(BF16, E4M3) : F(FP16, E4M3))         \
                           : ((type) == Type::kBF16 ? F(BF16, BF16) : F(FP16, FP16)))
+
+// The head dim that kernels compute with: 64, 128 or 256.
+inline int padded_dim(int dim) { return dim <= 64 ? 64 : (dim <= 128 ? 128 : 256); }
+#define PAGED_DIM(dim, F, X, C) ((dim) <= 64 ? F(X, C, 64) : ((dim) <= 128 ? F(X, C, 128) : F(X, C, 256)))
 
 }  // namespace paged

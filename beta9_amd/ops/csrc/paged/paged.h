@@ -67,8 +67,8 @@ struct AttendArgs {
   const void* v_cache;
   const int* tables;
   const int* kv_lens;
-  const int* cu_new;  // null: row r is the one new token of request r
-  int64_t q_row, q_head, out_row, out_head, table_stride;
+  const int* cu_new;  // of a prompt
+  int64_t q_row, q_head, out_row, out_head, table_stride;  // out has no gaps
   int rows, requests, heads, kv_heads, dim, page_log2, width, pages;
   float score_scale;  // softmax scale * scale of the keys * log2(e): exponentials are taken to the base 2
   float value_scale;
@@ -80,13 +80,10 @@ struct AttendArgs {
 hipError_t launch_plan(const PlanArgs& a, hipStream_t stream);
 hipError_t launch_release(const ReleaseArgs& a, hipStream_t stream);
 hipError_t launch_write(const WriteArgs& a, hipStream_t stream);
-// For head dims of 64 and 128; workspace: as many floats as decode_workspace says.
-bool decode_takes(const AttendArgs& a);
+// workspace: as many floats as the function before says
 int64_t decode_workspace(const AttendArgs& a);
 hipError_t launch_decode(const AttendArgs& a, float* workspace, hipStream_t stream);
-bool prompt_takes(const AttendArgs& a);
 int64_t prompt_workspace(const AttendArgs& a);
 hipError_t launch_prompt(const AttendArgs& a, float* workspace, hipStream_t stream);
-hipError_t launch_attend_rows(const AttendArgs& a, hipStream_t stream);
 
 }  // namespace paged

@@ -72,9 +72,12 @@ __device__ inline u32x2 read_turned(const char* p) {
 
 // 16 bytes a lane from `from` + `at` bytes to LDS at `to` + 16 * lane. By hand, since the compiler takes a transposing read
 // of LDS for one that may meet any load into LDS on its way, and would wait for the next tile there. It writes no register,
-// and what it brings is read after a wait for it and a barrier.
+// and what it brings is read after a wait for it and a barrier. The five steps between a lane's value moved to a scalar
+// register and a memory instruction that uses it are waited here too.
 __device__ inline void load_into_lds(const char* from, uint32_t at, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(at), "s"(from), "s"(to) : "memory", "m0");
+  uint64_t address = (uint64_t)from;
+  address = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(address >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)address);
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(at), "s"(address), "s"(__builtin_amdgcn_readfirstlane(to)) : "memory", "m0");
 }
 
 template <int N> struct Constant {
@@ -163,8 +166,9 @@ __device__ inline Where where_of(const PromptArgs& s, int item, bool whole) {
   return {-1, 0, 0, 0, 0, 0, 1, 0, 0};
 }
 
-template <class X, class C, int D>
-__global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : 2) void prompt_kernel(PromptArgs s) {
+// D: 64, 128 or 256. A smaller head dim takes the next of these (kPad): what lies past it is zero in LDS and in q.
+template <class X, class C, int D, bool kPad>
+__global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : (D == 128 ? 2 : 1)) void prompt_kernel(PromptArgs s) {
   typedef typename Vec<X>::x8 Half8;
   typedef typename X::T Out;
   constexpr bool kNarrow = sizeof(typename C::T) == 1;
@@ -175,6 +179,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : 2) void prompt_kernel(Pr
   constexpr int kRowBytes = D * 2, kChunks = D / 8, kTileBytes = kKeys * kRowBytes;
   __shared__ __attribute__((aligned(16))) char lds[2 * 2 * kTileBytes];  // [K, V][buffer][key][dim]
   const AttendArgs& a = s.a;
+  const int dim = kPad ? a.dim : D;
   int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5, n = lane & 31;
   int item = s.kv_heads_log2 >= 0 ? blockIdx.x >> s.kv_heads_log2 : blockIdx.x / a.kv_heads, kv_head = blockIdx.x - item * a.kv_heads;
 
@@ -184,9 +189,13 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : 2) void prompt_kernel(Pr
     rest = clamp_int(rest, 0, a.rows), front = clamp_int(front, 0, a.rows);
     for (int64_t r = blockIdx.x; r < front + (int64_t)a.rows - rest; r += gridDim.x) {
       Out* out = (Out*)a.out + (r < front ? r : r - front + rest) * a.out_row;
-      for (int i = tid; i < a.heads * D; i += kWaves * 64) out[(i / D) * a.out_head + i % D] = (Out)0.f;
+      for (int i = tid; i < a.heads * dim; i += kWaves * 64) out[i] = (Out)0.f;
     }
   };
+  if constexpr (kPad && !kNarrow) {  // what no load writes
+    for (int i = tid; i < 4 * kTileBytes / 16; i += kWaves * 64) reinterpret_cast<u32x4*>(lds)[i] = u32x4{};
+    __syncthreads();
+  }
   Where w = where_of(s, item, false);
   if (w.request < 0) {
     clear_rest();
@@ -218,20 +227,31 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : 2) void prompt_kernel(Pr
   };
   // which chunk of a key's row lies at place 0: differs for the 16 rows that a read of K covers, and by more than the pairs
   // that a read of V covers for four neighbouring rows
-  auto swizzle = [](int key) { return D == 128 ? (key & 3) << 2 | (key >> 2 & 3) : (key & 2) << 1 | (key >> 2 & 3); };
+  auto swizzle = [](int key) { return D == 64 ? (key & 2) << 1 | (key >> 2 & 3) : (key & 3) << 2 | (key >> 2 & 3); };
 
   // 16-bit: straight into LDS, 1 KB an instruction, which lie in one page; the lanes fetch what belongs at their place
   constexpr int kPieceKeys = 1024 / kRowBytes, kPieces = kTileBytes / 1024 / kWaves;
   uint32_t lds_base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds) + wave * 1024;
   int piece_key = lane / kChunks;
-  uint32_t piece_at = piece_key * kRowBytes + (((lane % kChunks) ^ swizzle(wave * kPieceKeys + piece_key)) * 16);
+  // a piece four further on (and twice that at a head dim of 256, where a piece is two keys) has the same exchange of chunks
+  constexpr int kKinds = D == 256 ? 2 : 1;
+  uint32_t piece_at[kKinds];
+  bool piece_there[kKinds];
+#pragma unroll
+  for (int i = 0; i < kKinds; i++) {
+    int chunk = (lane % kChunks) ^ swizzle((wave + kWaves * i) * kPieceKeys + piece_key);
+    piece_at[i] = piece_key * dim * 2 + chunk * 16;
+    piece_there[i] = !kPad || chunk * 8 < dim;
+  }
   auto stage = [&](int side, int tile, int buffer, int entry) {
     uint32_t row = cache_row(entry, lane);  // the low bits of a key are its place in the tile: a tile begins on 64
     if (a.page_log2 > 6) row += (tile * kKeys) & in_page & ~(kKeys - 1);
 #pragma unroll
-    for (int i = 0; i < kPieces; i++)
-      load_into_lds(caches[side] + (uint64_t)(uint32_t)__builtin_amdgcn_readlane(row, (wave + kWaves * i) * kPieceKeys) * kRowBytes, piece_at,
-                    lds_base + (2 * side + buffer) * kTileBytes + kWaves * i * 1024);
+    for (int i = 0; i < kPieces; i++) {
+      const char* from = caches[side] + (uint64_t)(uint32_t)__builtin_amdgcn_readlane(row, (wave + kWaves * i) * kPieceKeys) * (dim * 2);
+      if (piece_there[i % kKinds])
+        load_into_lds(from, piece_at[i % kKinds], lds_base + (2 * side + buffer) * kTileBytes + kWaves * i * 1024);
+    }
   };
   // 8-bit: through registers, widened on the way to LDS
   constexpr int kUnits = kKeys * D / 16 / (kWaves * 64);  // 16 dims each
@@ -241,7 +261,15 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : 2) void prompt_kernel(Pr
     for (int i = 0; i < kUnits; i++) {
       int unit = tid + i * kWaves * 64, key = unit / (D / 16);
       uint64_t row = cache_row(__shfl(entry, key), tile * kKeys + key);
-      narrow[i] = *reinterpret_cast<const u32x4*>(caches[side] + row * D + (unit % (D / 16)) * 16);
+      int at = (unit % (D / 16)) * 16;
+      const char* from = caches[side] + row * dim + at;
+      if (!kPad || at + 16 <= dim) {
+        narrow[i] = *reinterpret_cast<const u32x4*>(from);
+      } else {
+        u32x2 x = {};
+        if (at + 8 <= dim) x = *reinterpret_cast<const u32x2*>(from);
+        narrow[i] = u32x4{x[0], x[1], 0, 0};
+      }
     }
   };
   auto put = [&](int side, int buffer) {
@@ -262,7 +290,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : 2) void prompt_kernel(Pr
 #pragma unroll
     for (int i = 0; i < kSteps; i++) {
       Half8 x = {};
-      if (real) {
+      if (real && (!kPad || half * 8 + 16 * i < dim)) {
         if (s.q_wide) {
           x = *reinterpret_cast<const Half8*>(p + 16 * i);
         } else {
@@ -565,7 +593,8 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : 2) void prompt_kernel(Pr
     int from = i * (64 / kChunks) + lane / kChunks, chunk = lane % kChunks;
     int to = __shfl(place, from);
     u32x4 y = *reinterpret_cast<const u32x4*>(mine + from * kRowBytes + chunk * 16);
-    if (to >= 0) *reinterpret_cast<u32x4*>((Out*)a.out + (int64_t)to * D + (chunk ^ (from & (kChunks - 1))) * 8) = y;
+    int at = (chunk ^ (from & (kChunks - 1))) * 8;
+    if (to >= 0 && (!kPad || at < dim)) *reinterpret_cast<u32x4*>((Out*)a.out + (int64_t)to * dim + at) = y;
   }
 }
 
@@ -578,7 +607,7 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs s) {
   if (w.request < 0 || w.parts <= 1) return;
   constexpr int kLanes = D / 4, kAhead = 8;
   int dim = (threadIdx.x % kLanes) * 4, r = blockIdx.y * (256 / kLanes) + threadIdx.x / kLanes, row = w.tile * kRows + r;
-  if (row >= w.rows * s.group) return;
+  if (row >= w.rows * s.group || dim >= a.dim) return;
   float m = kMinusInf, l = 0.f;
   f32x4 o = {};
   for (int i = 0; i < w.parts; i += kAhead) {
@@ -622,11 +651,9 @@ int split_log2_of(const AttendArgs& a) {
 
 }  // namespace
 
-bool prompt_takes(const AttendArgs& a) { return a.dim == 64 || a.dim == 128; }
-
 int64_t prompt_workspace(const AttendArgs& a) {
   int log2 = split_log2_of(a);
-  return log2 < 0 ? 0 : (tiles_of(a) + (1LL << log2)) * a.kv_heads * kRows * (a.dim + 2);
+  return log2 < 0 ? 0 : (tiles_of(a) + (1LL << log2)) * a.kv_heads * kRows * (padded_dim(a.dim) + 2);
 }
 
 hipError_t launch_prompt(const AttendArgs& a, float* workspace, hipStream_t stream) {
@@ -642,16 +669,19 @@ hipError_t launch_prompt(const AttendArgs& a, float* workspace, hipStream_t stre
   if (items < 1) items = 1;
   s.target_log2 = split_log2_of(a);
   if (s.target_log2 >= 0) items += 1LL << s.target_log2;
-  s.part = workspace, s.stats = workspace + items * a.kv_heads * kRows * a.dim;
+  s.part = workspace, s.stats = workspace + items * a.kv_heads * kRows * padded_dim(a.dim);
   if (items * a.kv_heads >= (1LL << 31)) return hipErrorInvalidValue;
   dim3 grid((unsigned)(items * a.kv_heads));
-#define LAUNCH(X, C) (a.dim == 64 ? launch(prompt_kernel<X, C, 64>, grid, kWaves * 64, stream, s) : launch(prompt_kernel<X, C, 128>, grid, kWaves * 64, stream, s))
+#define LAUNCH_DIM(X, C, D) (a.dim == D ? launch(prompt_kernel<X, C, D, false>, grid, kWaves * 64, stream, s) : launch(prompt_kernel<X, C, D, true>, grid, kWaves * 64, stream, s))
+#define LAUNCH(X, C) PAGED_DIM(a.dim, LAUNCH_DIM, X, C)
   hipError_t status = PAGED_DISPATCH(a.type, a.cache, LAUNCH);
 #undef LAUNCH
+#undef LAUNCH_DIM
   if (status != hipSuccess || s.target_log2 < 0 || !tiles) return status;
-  dim3 joins((unsigned)(tiles * a.kv_heads), kRows / (256 / (a.dim / 4)));
-  if (a.type == Type::kBF16) return a.dim == 64 ? launch(prompt_join_kernel<BF16, 64>, joins, 256, stream, s) : launch(prompt_join_kernel<BF16, 128>, joins, 256, stream, s);
-  return a.dim == 64 ? launch(prompt_join_kernel<FP16, 64>, joins, 256, stream, s) : launch(prompt_join_kernel<FP16, 128>, joins, 256, stream, s);
+  dim3 joins((unsigned)(tiles * a.kv_heads), kRows / (256 / (padded_dim(a.dim) / 4)));
+#define LAUNCH_DIM(X, C, D) launch(prompt_join_kernel<X, D>, joins, 256, stream, s)
+  return a.type == Type::kBF16 ? PAGED_DIM(a.dim, LAUNCH_DIM, BF16, BF16) : PAGED_DIM(a.dim, LAUNCH_DIM, FP16, FP16);
+#undef LAUNCH_DIM
 }
 
 }  // namespace paged

@@ -12,7 +12,8 @@ Four operators and the cache object that holds their state:
 
 The cache holds keys and values as [pages, kv heads, page size, head dim],
 in the type of the queries (bfloat16, float16) or in float8_e4m3fn with one
-scale each for keys and values. ``tables[r, i]`` is the page of request r's
+scale each for keys and values. Head dims are multiples of 8 up to 256; the
+attention kernels compute with 64, 128 or 256, so that these cost least. ``tables[r, i]`` is the page of request r's
 tokens i * page_size and on. Lengths, tables and slots stay on the GPU: no
 call copies to the host or waits, and every one can be captured into a HIP
 graph. Workspaces belong to the call, so calls on several streams, or from

@@ -37,7 +37,7 @@ setup(
             name="beta9_amd.ops._paged_ext",
             sources=[
                 os.path.join(CSRC, "paged", name)
-                for name in ("bind.cpp", "tables.hip", "write.hip", "rows.hip", "decode.hip", "prompt.hip")
+                for name in ("bind.cpp", "tables.hip", "write.hip", "decode.hip", "prompt.hip")
             ],
             extra_compile_args={"cxx": ext_flags, "nvcc": hip_flags},
         ),

@@ -354,16 +354,33 @@ def test_prompt_attention_over_many_tiles(device, kind, cached, dim, page):
 
 
 @both
-@pytest.mark.parametrize("kind,cached", KINDS)
-@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 4, 4), (128, 8, 2), (128, 5, 1), (64, 40, 1)])
+@pytest.mark.parametrize("cached", ["bf16", "e4m3"])
+@pytest.mark.parametrize("dim", range(8, 257, 8))
+def test_every_head_dim(device, dim, cached):
+    """Decode split and joined, prompts in tiles and with split keys; the cache's neighbours hold no numbers."""
+    gen = torch.Generator().manual_seed(dim)
+    lens, new = [700, 0, 65], [70, 0, 3]
+    cu = [0, 70, 70, 73]
+    cache = make_cache(gen, lens, 2, dim, 64, "bf16", cached, device)
+    wide = (cache[0], cache[1], [t + [0] * 20 for t in cache[2]], cache[3])  # room for more keys: split and joined
+    q = torch.randn((73, 4, dim), generator=gen).to(torch.bfloat16).to(device)
+    for c in (cache, wide):
+        check_attention(run_decode(q[:3], c, lens), q[:3], cache, lens, [0, 1, 2, 3])
+        check_attention(run_prompt(q, c, lens, cu), q, cache, lens, cu)
+
+
+FEW = [([7], [3000]), ([1, 0, 40, 3], [2500, 900, 0, 1023]), ([130], [1100])]
+MANY = ([2] * 70, [600 + 13 * i for i in range(70)])
+
+
+@both
 @pytest.mark.parametrize(
-    "new,held",
-    [([7], [3000]), ([1, 0, 40, 3], [2500, 900, 0, 1023]), ([130], [1100]), ([2] * 70, [600 + 13 * i for i in range(70)])],
+    "kind,cached,dim,heads,kv_heads,new,held",
+    [(*k, *d, *x) for k in KINDS for d in [(64, 4, 4), (128, 8, 2), (128, 5, 1), (64, 40, 1)] for x in FEW]
+    + [("bf16", "bf16", 128, 8, 2, *MANY)],
 )
 def test_prompt_attention_of_few_rows_over_many_keys(device, kind, cached, dim, heads, kv_heads, new, held):
     """The last tokens of a request behind a long beginning, one, several and more than 64 requests."""
-    if len(new) > 4 and (heads, kind, cached) != (8, "bf16", "bf16"):
-        pytest.skip("once is enough")
     gen = torch.Generator().manual_seed(len(new) + dim)
     lens = [h + n for h, n in zip(held, new)]
     cu = [0]
