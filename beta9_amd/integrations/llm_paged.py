@@ -71,6 +71,8 @@ class PagedDecoder:
                 f"kv_cache={args.kv_cache!r} needs full attention in every layer and a head dim that is a "
                 f"multiple of 8 up to {MAX_HEAD_DIM}; this model has {sorted(kinds)} and {dim}"
             )
+        if device != "cpu" and dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"kv_cache={args.kv_cache!r} needs dtype='bfloat16' on a GPU, not {args.dtype!r}")
         model.set_attn_implementation(register())
         self.model, self.args, self.eos_id, self.device = model, args, eos_id, device
         size = args.kv_page_size

@@ -90,6 +90,7 @@ std::vector<Tensor> plan_step(const Tensor& tables, const Tensor& lens, const Te
   check_table(tables, tables, page_size);
   int64_t n = tables.size(0);
   REQUIRE(n >= 1, "tables must have a row");
+  REQUIRE(n == 1 || tables.stride(0) >= tables.size(1), "the rows of tables must not overlap");
   check_ints(lens, tables, 1, "lens");
   check_ints(new_lens, tables, 1, "new_lens");
   check_ints(free_pages, tables, 1, "free_pages");
@@ -121,6 +122,7 @@ std::vector<Tensor> release_pages(const Tensor& tables, const Tensor& lens, cons
   check_table(tables, tables, page_size);
   int64_t n = tables.size(0);
   REQUIRE(n >= 1, "tables must have a row");
+  REQUIRE(n == 1 || tables.stride(0) >= tables.size(1), "the rows of tables must not overlap");
   check_ints(lens, tables, 1, "lens");
   check_ints(free_pages, tables, 1, "free_pages");
   check_ints(free_count, tables, 1, "free_count");

@@ -13,8 +13,9 @@ Four operators and the cache object that holds their state:
 The cache holds keys and values as [pages, kv heads, page size, head dim],
 in the type of the queries (bfloat16, float16) or in float8_e4m3fn with one
 scale each for keys and values. Head dims are multiples of 8 up to 256; the
-attention kernels compute with 64, 128 or 256, so that these cost least. ``tables[r, i]`` is the page of request r's
-tokens i * page_size and on. Lengths, tables and slots stay on the GPU: no
+attention kernels compute with 64, 128 or 256, so these cost least. Page
+sizes are 16 to 256 in powers of two. ``tables[r, i]`` is the page of request
+r's tokens i * page_size and on. Lengths, tables and slots stay on the GPU: no
 call copies to the host or waits, and every one can be captured into a HIP
 graph. Workspaces belong to the call, so calls on several streams, or from
 several captured graphs, share nothing but the tensors they are given.
@@ -28,6 +29,7 @@ hard error, and CPU tensors take a plain torch path (any floating type).
 from __future__ import annotations
 
 import math
+import threading
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -40,22 +42,25 @@ PAGE_SIZES = (16, 32, 64, 128, 256)
 
 _ext = None
 _tried = False
+_loading = threading.Lock()
 
 
 def _load():
     global _ext, _tried
     if not _tried:
-        _tried = True
-        try:
-            from . import _paged_ext
+        with _loading:  # a second thread's first call waits for the import
+            if not _tried:
+                try:
+                    from . import _paged_ext
 
-            _ext = _paged_ext
-        except ImportError as e:
-            if torch.cuda.is_available():
-                raise RuntimeError(
-                    f"gfx950 paged-cache extension missing on a GPU host: {e}; "
-                    "run __graft_entry__.build()"
-                )
+                    _ext = _paged_ext
+                except ImportError as e:
+                    if torch.cuda.is_available():
+                        raise RuntimeError(
+                            f"gfx950 paged-cache extension missing on a GPU host: {e}; "
+                            "run __graft_entry__.build()"
+                        )
+                _tried = True
     return _ext
 
 
@@ -341,6 +346,7 @@ def _check_stack(tables, lens, other, name, free_pages, free_count, page_size) -
     _check_table(tables, tables, page_size)
     n = tables.shape[0]
     _require(n >= 1, "tables must have a row")
+    _require(n == 1 or tables.stride(0) >= tables.shape[1], "the rows of tables must not overlap")
     _check_ints(lens, tables, 1, "lens")
     _check_ints(free_pages, tables, 1, "free_pages")
     _check_ints(free_count, tables, 1, "free_count")

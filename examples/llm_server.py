@@ -11,7 +11,7 @@ from beta9_amd.integrations import LLM, LLMArgs
 
 llm = LLM(
     args=LLMArgs(model="synthetic-llama", hidden_size=1024, num_hidden_layers=8,
-                 max_num_seqs=32),
+                 max_num_seqs=32, kv_cache="paged"),
     gpu="MI355X",
     cpu=4000,
     memory=16384,

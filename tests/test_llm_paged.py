@@ -107,6 +107,9 @@ def test_paged_refusals():
         LLMEngine(args(kv_cache="paged", hidden_size=48, num_attention_heads=4))
     with pytest.raises(ValueError, match="page_size"):
         LLMEngine(args(kv_cache="paged", kv_page_size=17))
+    if torch.cuda.is_available():
+        with pytest.raises(ValueError, match="dtype"):
+            LLMEngine(args(kv_cache="paged", dtype="float32"))
     engine = LLMEngine(args(kv_cache="paged"))
     got, errors = ids_of(engine, ["hello", "ok"], [0, 2])
     assert got[0] == [] and errors == [None, None] and len(got[1]) in (1, 2)

@@ -664,6 +664,7 @@ def test_write_refusals(device, change, error):
         (dict(tables=lambda x: x.float()), TypeError),
         (dict(tables=lambda x: x[:0]), ValueError),
         (dict(tables=lambda x: x.repeat(3000, 1)), ValueError),
+        (dict(tables=lambda x: x[:1].expand(2, 2)), ValueError),
         (dict(lens=lambda x: x[:1]), ValueError),
         (dict(lens=lambda x: x.long()), TypeError),
         (dict(new_lens=lambda x: x[:1]), ValueError),
