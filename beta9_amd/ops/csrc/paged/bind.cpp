@@ -62,6 +62,7 @@ Type check_caches(const Tensor& k, const Tensor& v, const Tensor& like, Type typ
                    "k_cache and v_cache must both be ", like.scalar_type(), " or float8_e4m3fn");
   REQUIRE(k.size(0) >= 1 && k.size(1) >= 1, "the cache must have a page and a head");
   REQUIRE(k.size(0) * k.size(2) < (1LL << 31), "the cache must have fewer than 2^31 slots");
+  REQUIRE(k.size(0) * k.size(2) * k.size(1) < (1LL << 32), "the cache must have fewer than 2^32 rows of a head");
   REQUIRE(k.size(3) % 8 == 0 && k.size(3) >= 8 && k.size(3) <= paged::kMaxHeadDim, "head dim must be a multiple of 8, at most ",
           paged::kMaxHeadDim, ", is ", k.size(3));
   return k.scalar_type() == at::kFloat8_e4m3fn ? Type::kE4M3 : type;

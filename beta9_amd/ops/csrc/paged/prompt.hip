@@ -223,7 +223,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : (D == 128 ? 2 : 1)) void
   auto entry_of = [&](int tile) { return table[min((tile * kKeys + lane) >> a.page_log2, a.width - 1)]; };
   auto cache_row = [&](int entry, int key) {
     uint32_t page = (unsigned)entry < (unsigned)a.pages ? entry : 0;
-    return ((page * a.kv_heads + kv_head) << a.page_log2) + (key & in_page);  // memory holds fewer than 2^32 rows
+    return ((page * a.kv_heads + kv_head) << a.page_log2) + (key & in_page);  // fits: the cache has fewer than 2^32 rows
   };
   // which chunk of a key's row lies at place 0: differs for the 16 rows that a read of K covers, and by more than the pairs
   // that a read of V covers for four neighbouring rows

@@ -376,6 +376,7 @@ def _check_caches(k_cache, v_cache, like) -> None:
     _page_size(page_size)
     _require(pages >= 1 and heads >= 1, "the cache must have a page and a head")
     _require(pages * page_size < 2**31, "the cache must have fewer than 2^31 slots")
+    _require(pages * page_size * heads < 2**32, "the cache must have fewer than 2^32 rows of a head")
     _require(
         dim % 8 == 0 and 8 <= dim <= MAX_HEAD_DIM,
         f"head dim must be a multiple of 8, at most {MAX_HEAD_DIM}, is {dim}",
