@@ -28,11 +28,25 @@ constexpr int kWaves = 4;
 constexpr int kRows = 32 * kWaves;
 constexpr int kKeys = 64;
 
+// x / d for 0 <= x < 2^31 by a product: with 2^(L - 1) < d <= 2^L, m = floor(2^(31 + L) / d) + 1 is more than 2^(31 + L) / d by
+// at most 1, so x m / 2^(31 + L) exceeds x / d by less than 1 / d.
+struct Divisor {
+  uint32_t m, shift;
+  explicit Divisor(uint32_t d = 1) {
+    uint32_t log2 = 0;
+    while ((1u << log2) < d) log2++;
+    shift = 31 + log2;
+    m = (uint32_t)((1ull << shift) / d + 1);
+  }
+  __device__ int divide(int x) const { return (int)((uint64_t)(uint32_t)x * m >> shift); }
+};
+
 struct PromptArgs {
   AttendArgs a;
   int q_wide;    // q's rows begin on 16 bytes
   int negative;  // the scale is below zero: q's sign is turned instead
-  int group, group_log2, kv_heads_log2;  // logarithms: -1 where there is none
+  int group;
+  Divisor by_group, by_kv_heads;
   int target_log2;  // chunks of keys wanted for all tiles of a kv head together; -1: keys are not split
   float* part;      // [items, kv heads, kRows, dim]: unnormalised sums
   float* stats;     // [items, kv heads, kRows, 2]: running maximum and sum
@@ -181,7 +195,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : (D == 128 ? 2 : 1)) void
   const AttendArgs& a = s.a;
   const int dim = kPad ? a.dim : D;
   int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5, n = lane & 31;
-  int item = s.kv_heads_log2 >= 0 ? blockIdx.x >> s.kv_heads_log2 : blockIdx.x / a.kv_heads, kv_head = blockIdx.x - item * a.kv_heads;
+  int item = s.by_kv_heads.divide(blockIdx.x), kv_head = blockIdx.x - item * a.kv_heads;
 
   int rest = a.cu_new[a.requests], front = a.cu_new[0];  // on their way while the rest goes on
   auto clear_rest = [&]() {
@@ -202,7 +216,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : (D == 128 ? 2 : 1)) void
     return;
   }
   int group = s.group;
-  auto by_group = [&](int x) { return s.group_log2 >= 0 ? x >> s.group_log2 : x / group; };
+  auto by_group = [&](int x) { return s.by_group.divide(x); };
   int packed = w.rows * group;  // fits: rows by heads do
   int length = w.keys;
   int ahead = length - w.rows;  // a token's position less its number among the new ones
@@ -602,7 +616,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : (D == 128 ? 2 : 1)) void
 template <class X, int D>
 __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs s) {
   const AttendArgs& a = s.a;
-  int item = blockIdx.x / a.kv_heads, kv_head = blockIdx.x - item * a.kv_heads;
+  int item = s.by_kv_heads.divide(blockIdx.x), kv_head = blockIdx.x - item * a.kv_heads;
   Where w = where_of(s, item, true);
   if (w.request < 0 || w.parts <= 1) return;
   constexpr int kLanes = D / 4, kAhead = 8;
@@ -627,7 +641,7 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs s) {
       m = top;
     }
   }
-  int token = row / s.group, head = kv_head * s.group + row - token * s.group;
+  int token = s.by_group.divide(row), head = kv_head * s.group + row - token * s.group;
   typename X::T* out = (typename X::T*)a.out + (w.row0 + token) * a.out_row + head * a.out_head + dim;
   float f = l == 0.f ? 0.f : a.value_scale / l;
   typename Vec<X>::x4 y;
@@ -663,8 +677,7 @@ hipError_t launch_prompt(const AttendArgs& a, float* workspace, hipStream_t stre
   s.negative = a.score_scale < 0;
   // a scale of zero weighs all keys alike, as does one that small, and spares the kernel -inf * 0
   s.a.score_scale = a.score_scale == 0 ? 0x1p-100f : (s.negative ? -a.score_scale : a.score_scale);
-  auto log2 = [](int x) { return x & (x - 1) ? -1 : __builtin_ctz(x); };
-  s.group = a.heads / a.kv_heads, s.group_log2 = log2(s.group), s.kv_heads_log2 = log2(a.kv_heads);
+  s.group = a.heads / a.kv_heads, s.by_group = Divisor(s.group), s.by_kv_heads = Divisor(a.kv_heads);
   int64_t tiles = tiles_of(a), items = tiles;
   if (items < 1) items = 1;
   s.target_log2 = split_log2_of(a);
