@@ -107,7 +107,7 @@ struct Where {
 // Which rows the item stands for. The tiles that see the most keys come first, so that the last workgroups to start are
 // short ones: up to 64 requests, all tiles are put in order of their last position, in 64 steps (a lane a step counts the
 // tiles in it); among more, the requests follow each other, each from its last tile to its first. On 13 ragged prompts
-// (16 heads of 64, up to 1500 new tokens) 75.8 us, in the requests' order 77.9.
+// (16 heads of 64, up to 1500 new tokens) 71.0 us, in the requests' order 83.1.
 //
 // If there are few tiles, their keys are split: into chunks that are equal for all requests, as for one token. A request's
 // tiles have as many parts as its last one needs; the parts of earlier tiles that hold no keys add nothing. `whole`: the item
@@ -180,9 +180,14 @@ __device__ inline Where where_of(const PromptArgs& s, int item, bool whole) {
   return {-1, 0, 0, 0, 0, 0, 1, 0, 0};
 }
 
+// Waves of a SIMD, for the registers that they may have. At a head dim of 64 the pass over the keys takes 120, a narrow
+// cache's more; the careful pass, in the same kernel, takes 168 and keeps some in memory for the fourth wave's sake (13 prompts
+// of up to 1500 tokens, 16 heads of 64: 70.6 us with four waves, 75.0 with three; 4 of 8192: 668 and 705).
+constexpr int waves_of(int dim, bool narrow) { return dim == 64 ? (narrow ? 3 : 4) : (dim == 128 ? 2 : 1); }
+
 // D: 64, 128 or 256. A smaller head dim takes the next of these (kPad): what lies past it is zero in LDS and in q.
 template <class X, class C, int D, bool kPad>
-__global__ __launch_bounds__(kWaves * 64, D == 64 ? 3 : (D == 128 ? 2 : 1)) void prompt_kernel(PromptArgs s) {
+__global__ __launch_bounds__(kWaves * 64, waves_of(D, sizeof(typename C::T) == 1)) void prompt_kernel(PromptArgs s) {
   typedef typename Vec<X>::x8 Half8;
   typedef typename X::T Out;
   constexpr bool kNarrow = sizeof(typename C::T) == 1;
