@@ -99,7 +99,8 @@ template <int N> struct Constant {
 };
 
 struct Where {
-  int request, tile, row0, rows, keys;  // the request's first packed row, its new tokens and all of them
+  int request, tile, row0, rows, keys;  // the request's first packed row, its new tokens (as far as there are rows) and all of them
+  int ahead;                            // a token's position less its number among the new ones
   int part, parts, chunk;               // of its keys, the part and its length in tiles of keys
   int index;                            // where the first of the rows' parts lies in the workspace
 };
@@ -116,16 +117,16 @@ __device__ inline Where where_of(const PromptArgs& s, int item, bool whole) {
   const AttendArgs& a = s.a;
   int lane = threadIdx.x & 63, before = 0, items_before = 0;
   struct Request {
-    int row0, n, keys, tiles;
+    int row0, until, keys, tiles;
   };
   auto request = [&](int i) {
     Request r = {0, 0, 0, 0};
     if (i < a.requests) {
       r.row0 = clamp_int(a.cu_new[i], 0, a.rows);
-      r.n = clamp_int(a.cu_new[i + 1], r.row0, a.rows) - r.row0;
+      r.until = max(a.cu_new[i + 1], r.row0);
       r.keys = clamp_int(a.kv_lens[i], 0, a.width << a.page_log2);
     }
-    r.tiles = (int)(((int64_t)r.n * s.group + kRows - 1) / kRows);
+    r.tiles = (int)(((int64_t)(min(r.until, a.rows) - r.row0) * s.group + kRows - 1) / kRows);
     return r;
   };
   Request mine = request(lane);
@@ -148,7 +149,7 @@ __device__ inline Where where_of(const PromptArgs& s, int item, bool whole) {
       count = whole ? r.tiles : r.tiles * parts;
     } else if (a.requests > 1 && a.requests <= 64) {
       // in tiles' places: the request's begin behind what it held before
-      int start = (int)(min((int64_t)max(r.keys - r.n, 0) * s.group, (int64_t)1 << 30) / kRows), end = start + r.tiles;
+      int start = (int)(min((int64_t)max(r.keys - (r.until - r.row0), 0) * s.group, (int64_t)1 << 30) / kRows), end = start + r.tiles;
       int width = (whole_max(end) + 63) / 64, low = (63 - lane) * width, here = 0;
       for (int i = 0; i < a.requests; i++)
         here += clamp_int(lane_value(end, i) - low, 0, width) - clamp_int(lane_value(start, i) - low, 0, width);
@@ -165,7 +166,8 @@ __device__ inline Where where_of(const PromptArgs& s, int item, bool whole) {
     uint64_t found = __ballot(before + up > item);
     if (found) {
       int at = __builtin_ctzll(found), local = item - before - lane_value(up - count, at);
-      Where w = {first + at, 0, lane_value(r.row0, at), lane_value(r.n, at), lane_value(r.keys, at), 0, lane_value(parts, at), chunk, 0};
+      int row0 = lane_value(r.row0, at), until = lane_value(r.until, at), keys = lane_value(r.keys, at);
+      Where w = {first + at, 0, row0, min(until, a.rows) - row0, keys, keys - (until - row0), 0, lane_value(parts, at), chunk, 0};
       int back = chunk && !whole ? local / w.parts : local;  // tiles from the last
       w.tile = lane_value(from + count, at) - 1 - back;
       if (chunk) {
@@ -224,7 +226,7 @@ __global__ __launch_bounds__(kWaves * 64, waves_of(D, sizeof(typename C::T) == 1
   auto by_group = [&](int x) { return s.by_group.divide(x); };
   int packed = w.rows * group;  // fits: rows by heads do
   int length = w.keys;
-  int ahead = length - w.rows;  // a token's position less its number among the new ones
+  int ahead = w.ahead;
   int row_first = w.tile * kRows, wave_first = row_first + wave * 32;
   int row = wave_first + n;
   bool real = row < packed;

@@ -445,6 +445,21 @@ def test_lengths_past_the_table_end_with_it(device, dim):
 
 @both
 @pytest.mark.parametrize("dim", [80, 64, 128])
+@pytest.mark.parametrize("rows", [1, 30, 41, 160])
+def test_fewer_rows_than_new_tokens(device, dim, rows):
+    """The first rows of a step: what each of them sees does not change."""
+    gen = torch.Generator().manual_seed(rows)
+    lens, cu = [90, 100, 700], [0, 40, 140, 170]
+    cache = make_cache(gen, lens, 2, dim, 16, "bf16", "bf16", device)
+    q = torch.randn((170, 4, dim), generator=gen).to(torch.bfloat16).to(device)
+    want, off = attention_oracle(q, *cache[:3], lens, cu, dim**-0.5, *cache[3])
+    got = run_prompt(q[:rows], cache, lens, cu)
+    assert got.shape[0] == rows
+    assert ((got.cpu().double() - want[:rows]).abs() <= off[:rows]).all()
+
+
+@both
+@pytest.mark.parametrize("dim", [80, 64, 128])
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
 def test_later_tokens_do_not_reach_earlier_rows(device, dim, bad):
     """A value or key that is not finite changes the rows that see it and no others."""
