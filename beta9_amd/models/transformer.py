@@ -155,6 +155,8 @@ class TransformerServingModel:
 
     def infer_decode(self, requests: int = 32, prompt_tokens: int = 256, steps: int = 16) -> Dict:
         """Prompts of ``requests`` requests, then ``steps`` tokens of each."""
+        if min(requests, prompt_tokens, steps) < 1:
+            raise ValueError("requests, prompt_tokens and steps must be positive")
         cache = self.new_cache(requests, prompt_tokens + steps)
         sync = torch.cuda.synchronize if self.device.startswith("cuda") else (lambda: None)
         lens = torch.full((requests,), prompt_tokens, dtype=torch.int32, device=self.device)

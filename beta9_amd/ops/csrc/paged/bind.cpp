@@ -74,7 +74,10 @@ void check_table(const Tensor& tables, const Tensor& like, int64_t page_size) {
   REQUIRE(tables.size(1) >= 1 && tables.size(1) * page_size <= (1LL << 30), "a table row must name at least 1 and at most 2^30 slots");
 }
 
-void check_scale(double x, const char* name) { REQUIRE(std::isfinite(x) && x > 0, name, " must be a positive number, is ", x); }
+// The kernels multiply by it and by its inverse, in 32 bits.
+void check_scale(double x, const char* name) {
+  REQUIRE(x >= 0x1p-126 && x <= 0x1p126, name, " must be a positive number that fits 32 bits, and its inverse too, is ", x);
+}
 
 // A view of n values of a one-dimensional buffer, made directly: six of them by the dispatcher cost more than the launch.
 Tensor part_of(const Tensor& buffer, int64_t first, int64_t n) {
@@ -154,7 +157,8 @@ void write_kv(const Tensor& k, const Tensor& v, const Tensor& k_cache, const Ten
   a.page_log2 = page_log2(k_cache.size(2));
   REQUIRE(k.dim() == 3 && k.sizes() == v.sizes() && k.size(1) == k_cache.size(1) && k.size(2) == k_cache.size(3),
           "k and v must be [tokens, ", k_cache.size(1), ", ", k_cache.size(3), "] for this cache");
-  REQUIRE(k.size(0) < (1LL << 31), "too many tokens");
+  // a grid's threads are counted in 32 bits
+  REQUIRE(k.size(0) < (1LL << 31) && k.size(0) < (1LL << 32) / (k.size(1) * (k.size(2) / 8)), "too many tokens");
   REQUIRE(k.numel() == 0 || (k.stride(2) == 1 && v.stride(2) == 1), "k and v must have no gaps along the head dim");
   check_ints(slots, k, 1, "slots");
   REQUIRE(slots.size(0) == k.size(0), "slots must have one value for each of the ", k.size(0), " tokens, has ", slots.size(0));
@@ -193,7 +197,7 @@ Tensor attend(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, con
   } else {
     REQUIRE(q.size(0) == requests, "q must have one row for each of the ", requests, " rows of tables");
   }
-  REQUIRE(std::isfinite(scale), "scale must be finite");
+  REQUIRE(std::isfinite((float)(scale * k_scale * kLog2E)), "scale must be finite, also by k_scale in 32 bits");
   check_scale(k_scale, "k_scale");
   check_scale(v_scale, "v_scale");
   REQUIRE(a.cache == Type::kE4M3 || (k_scale == 1.0 && v_scale == 1.0), "only a float8_e4m3fn cache has scales");
@@ -219,6 +223,7 @@ Tensor attend(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, con
   a.width = (int)tables.size(1), a.pages = (int)k_cache.size(0);
   a.score_scale = (float)(scale * k_scale * kLog2E), a.value_scale = (float)v_scale;
   a.clear_rest = out_given ? 0 : 1;
+  REQUIRE(!cu_new || paged::prompt_fits(a), "too many rows, requests or heads");
   int64_t floats = cu_new ? paged::prompt_workspace(a) : paged::decode_workspace(a);
   Tensor workspace;
   if (floats) workspace = at::empty({floats}, q.options().dtype(at::kFloat));

@@ -84,6 +84,7 @@ hipError_t launch_write(const WriteArgs& a, hipStream_t stream);
 int64_t decode_workspace(const AttendArgs& a);
 hipError_t launch_decode(const AttendArgs& a, float* workspace, hipStream_t stream);
 int64_t prompt_workspace(const AttendArgs& a);
+bool prompt_fits(const AttendArgs& a);  // a grid's threads are counted in 32 bits
 hipError_t launch_prompt(const AttendArgs& a, float* workspace, hipStream_t stream);
 
 }  // namespace paged

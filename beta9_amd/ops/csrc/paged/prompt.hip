@@ -179,7 +179,7 @@ __device__ inline Where where_of(const PromptArgs& s, int item, bool whole) {
     }
     before += lane_value(up, 63), items_before += lane_value(items_up, 63);
   }
-  return {-1, 0, 0, 0, 0, 0, 1, 0, 0};
+  return {-1, 0, 0, 0, 0, 0, 0, 1, 0, 0};
 }
 
 // Waves of a SIMD, for the registers that they may have. At a head dim of 64 the pass over the keys takes 120, a narrow
@@ -672,6 +672,8 @@ int split_log2_of(const AttendArgs& a) {
 
 }  // namespace
 
+bool prompt_fits(const AttendArgs& a) { return (tiles_of(a) + kSplitBelow) * a.kv_heads < (1LL << 32) / (kWaves * 64); }
+
 int64_t prompt_workspace(const AttendArgs& a) {
   int log2 = split_log2_of(a);
   return log2 < 0 ? 0 : (tiles_of(a) + (1LL << log2)) * a.kv_heads * kRows * (padded_dim(a.dim) + 2);
@@ -690,7 +692,6 @@ hipError_t launch_prompt(const AttendArgs& a, float* workspace, hipStream_t stre
   s.target_log2 = split_log2_of(a);
   if (s.target_log2 >= 0) items += 1LL << s.target_log2;
   s.part = workspace, s.stats = workspace + items * a.kv_heads * kRows * padded_dim(a.dim);
-  if (items * a.kv_heads >= (1LL << 31)) return hipErrorInvalidValue;
   dim3 grid((unsigned)(items * a.kv_heads));
 #define LAUNCH_DIM(X, C, D) (a.dim == D ? launch(prompt_kernel<X, C, D, false>, grid, kWaves * 64, stream, s) : launch(prompt_kernel<X, C, D, true>, grid, kWaves * 64, stream, s))
 #define LAUNCH(X, C) PAGED_DIM(a.dim, LAUNCH_DIM, X, C)

@@ -107,9 +107,10 @@ def plan_step(
     last get slot -1.
 
     A request is served whole or not at all: it gets nothing if its row has
-    no room for its tokens, its rows pass ``num_tokens``, or the pages it
-    needs are more than the requests before it left. Its slots are then -1,
-    its kv_lens 0, and it holds what it held. New entries of ``tables`` are
+    no room for its tokens, its rows pass ``num_tokens``, or the stack has
+    too few pages for it and those before it; so once one finds too few,
+    none behind it that needs a page gets one. Its slots are then -1, its
+    kv_lens 0, and it holds what it held. New entries of ``tables`` are
     written in place; lens and free_count come back anew, so a step counts
     once the caller stores them (``PagedKVCache.plan`` does)."""
     ext = _native(tables)
@@ -151,7 +152,8 @@ def write_kv(
     whose slot is negative or past the cache are skipped. An 8-bit cache
     holds the value divided by its scale, clamped to +-448, rounded to the
     nearest. Slots must differ: which of two tokens with one slot stays is
-    not defined (``plan_step`` gives none twice)."""
+    not defined (``plan_step`` gives none twice). k and v must not lie in the
+    places that are written."""
     ext = _native(k)
     if ext is not None:
         ext.write_kv(k, v, k_cache, v_cache, slots, k_scale, v_scale)
@@ -240,11 +242,16 @@ class PagedKVCache:
         if min(layers, kv_heads, pages, requests, max_len) < 1:
             raise ValueError("layers, kv_heads, pages, requests and max_len must be positive")
         self.page_size, self.k_scale, self.v_scale = _page_size(page_size), k_scale, v_scale
+        shape = (layers, pages, kv_heads, page_size, head_dim)
+        like = torch.empty(shape, dtype=dtype, device="meta")
+        _check_caches(like[0], like[0], like[0])
+        _check_scales(like, k_scale, v_scale)
+        _check_table(torch.empty((requests, self.pages_for(max_len)), dtype=torch.int32, device="meta"), like, page_size)
         # zeros, not what the memory held: no page is read before it is written, but dumps and snapshots see all
-        self.k = torch.zeros((layers, pages, kv_heads, page_size, head_dim), dtype=dtype, device=device)
+        self.k = torch.zeros(shape, dtype=dtype, device=device)
         self.v = torch.zeros_like(self.k)
         ints = dict(dtype=torch.int32, device=device)
-        self.tables = torch.full((requests, -(-max_len // page_size)), -1, **ints)
+        self.tables = torch.full((requests, self.pages_for(max_len)), -1, **ints)
         self._state = torch.zeros(requests + 1, **ints)
         self._state[requests] = pages
         self.lens, self.free_count = self._state[:requests], self._state[requests:]
@@ -385,7 +392,9 @@ def _check_caches(k_cache, v_cache, like) -> None:
 
 def _check_scales(cache, k_scale, v_scale) -> None:
     for name, x in (("k_scale", k_scale), ("v_scale", v_scale)):
-        _require(math.isfinite(x) and x > 0, f"{name} must be a positive number, is {x}")
+        _require(
+            2.0**-126 <= x <= 2.0**126, f"{name} must be a positive number that fits 32 bits, and its inverse too, is {x}"
+        )
     _require(
         cache.dtype == torch.float8_e4m3fn or (k_scale == 1.0 and v_scale == 1.0),
         "only a float8_e4m3fn cache has scales",
@@ -454,6 +463,7 @@ def _write_plain(k, v, k_cache, v_cache, slots, k_scale, v_scale) -> None:
         k.dim() == 3 and k.shape == v.shape and k.shape[1:] == (heads, dim),
         f"k and v must be [tokens, {heads}, {dim}] for this cache",
     )
+    _require(k.shape[0] < min(2**31, 2**32 // (heads * (dim // 8))), "too many tokens")
     _require(
         k.numel() == 0 or (k.stride(2) == 1 and v.stride(2) == 1), "k and v must have no gaps along the head dim"
     )
@@ -481,7 +491,7 @@ def _attend_plain(q, k_cache, v_cache, tables, kv_lens, cu_new, scale, k_scale, 
     pages, kv_heads, page_size, dim = k_cache.shape
     _require(q.dim() == 3 and q.shape[2] == dim, f"q must be [rows, heads, {dim}] for this cache")
     rows, heads = q.shape[:2]
-    _require(heads <= 65535, "too many rows or heads")
+    _require(heads <= 65535 and (not heads or rows < 2**31 // heads), "too many rows or heads")
     _require(
         heads >= 1 and heads % kv_heads == 0, f"q's {heads} heads must be a multiple of the cache's {kv_heads}"
     )
@@ -495,10 +505,12 @@ def _attend_plain(q, k_cache, v_cache, tables, kv_lens, cu_new, scale, k_scale, 
     if cu_new is not None:
         _check_ints(cu_new, q, 1, "cu_new")
         _require(cu_new.shape[0] == requests + 1, f"cu_new must have {requests + 1} values, has {cu_new.shape[0]}")
+        tiles = rows * (heads // kv_heads) // 128 + requests
+        _require((tiles + 256) * kv_heads < 2**24, "too many rows, requests or heads")
     else:
         _require(rows == requests, f"q must have one row for each of the {requests} rows of tables")
-    _require(math.isfinite(scale), "scale must be finite")
     _check_scales(k_cache, k_scale, v_scale)
+    _require(abs(scale * k_scale * math.log2(math.e)) < 2.0**128, "scale must be finite, also by k_scale in 32 bits")
     if out is not None:
         _check(out, q, "out")
         _require(out.dtype == q.dtype, f"out must be {q.dtype} like q, is {out.dtype}", TypeError)

@@ -630,6 +630,42 @@ def test_attention_refusals(device, change, error):
 
 
 @both
+@pytest.mark.parametrize(
+    "more",
+    [dict(scale=1e39), dict(scale=-1e300), dict(k_scale=1e30, scale=1e10), dict(k_scale=1e-40), dict(v_scale=1e39), dict(v_scale=1e-50)],
+)
+def test_scales_that_32_bits_do_not_hold_are_refused(device, more):
+    args = good(device)
+    args["k_cache"], args["v_cache"] = (args[n].to(torch.float8_e4m3fn) for n in ("k_cache", "v_cache"))
+    cu = torch.zeros(4, dtype=torch.int32, device=device)
+    with pytest.raises(ValueError):
+        paged.decode_attention(*args.values(), **more)
+    with pytest.raises(ValueError):
+        paged.prompt_attention(*args.values(), cu, **more)
+    if "scale" not in more:
+        k = torch.zeros((2, 2, 64), dtype=torch.bfloat16, device=device)
+        with pytest.raises(ValueError):
+            paged.write_kv(k, k, args["k_cache"], args["v_cache"], ints([0, 1], device), **more)
+
+
+@both
+def test_more_work_than_a_launch_takes_is_refused(device):
+    """Sizes that take no memory: a row of each stands for all, or most requests bring nothing."""
+    bf16 = dict(dtype=torch.bfloat16, device=device)
+    cache = torch.zeros((1, 2048, 16, 8), **bf16)
+    tokens = 2**21
+    slots = ints([-1], device).repeat(tokens)
+    k = torch.zeros((1, 2048, 8), **bf16).expand(tokens, -1, -1)
+    with pytest.raises(ValueError, match="too many tokens"):
+        paged.write_kv(k, k, cache, cache, slots)
+    cache = torch.zeros((1, 8192, 16, 8), **bf16)
+    q = torch.zeros((1, 8192, 8), **bf16)
+    tables, lens, cu = ints([[0]], device).repeat(4096, 1), ints([0], device).repeat(4096), ints([0], device).repeat(4097)
+    with pytest.raises(ValueError, match="too many"):
+        paged.prompt_attention(q, cache, cache, tables, lens, cu)
+
+
+@both
 def test_head_dims_are_refused_that_no_kernel_takes(device):
     for dim in (4, 12, 264):
         q = torch.zeros((1, 1, dim), dtype=torch.bfloat16, device=device)
@@ -801,6 +837,12 @@ def test_cache_arguments(device):
         paged.PagedKVCache(1, 1, 64, 4, page_size=20, device=device)
     with pytest.raises(ValueError):
         paged.PagedKVCache(0, 1, 64, 4, device=device)
+    for more in (dict(head_dim=12), dict(head_dim=264), dict(requests=4097), dict(pages=2**27, page_size=16), dict(max_len=2**31)):
+        with pytest.raises(ValueError):
+            paged.PagedKVCache(**(dict(layers=1, kv_heads=1, head_dim=64, pages=4, device=device) | more))
+    for more in (dict(k_scale=0.5), dict(dtype=torch.float8_e4m3fn, v_scale=0.0)):
+        with pytest.raises(ValueError):
+            paged.PagedKVCache(1, 1, 64, 4, device=device, **more)
     cache = paged.PagedKVCache(1, 2, 64, 4, 16, 2, 40, device=device)
     assert cache.tables.shape == (2, 3) and cache.pages == 4 and cache.pages_for(17) == 2 and cache.k.dtype == torch.bfloat16
 
@@ -842,6 +884,27 @@ def test_transformer_model_over_the_cache(device):
 # -- streams, graphs, threads -----------------------------------------------
 
 gpu = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(), reason="needs MI355X")]
+
+
+@both
+def test_infer_decode(device, monkeypatch):
+    from beta9_amd.models import bench_handler
+    from beta9_amd.models.transformer import TransformerServingModel
+
+    torch.manual_seed(0)
+    model = TransformerServingModel(hidden=256, inter=512, layers=2, n_heads=4, n_kv_heads=2, device=device)
+    for b in model.blocks:
+        for w in (b.attn_norm, b.mlp_norm):
+            w.fill_(1.0)
+    monkeypatch.setattr(bench_handler, "_model", model)
+    r = bench_handler.infer(tokens=5, decode_steps=3, requests=2)
+    assert r["requests"] == 2 and r["tokens_per_sec"] > 0 and math.isfinite(r["checksum"])
+    for bad in ((0, 5, 3), (2, 0, 3), (2, 5, 0), (5000, 1, 1)):
+        with pytest.raises(ValueError):
+            model.infer_decode(*bad)
+    monkeypatch.setattr(bench_handler, "_model", object())
+    with pytest.raises(ValueError):
+        bench_handler.infer(tokens=5, decode_steps=3)
 
 
 class Loop:
