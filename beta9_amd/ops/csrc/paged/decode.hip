@@ -208,6 +208,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : 4) void split_kernel(Sp
 
   f32x4 acc[K::kPer] = {};
   float m = kMinusInf, l = 0.f;
+  uint64_t seen = 0;  // lanes that have had a key
   auto use = [&](typename K::Tile& t, int base) {
     f32x4 score[2] = {};
 #pragma unroll
@@ -219,6 +220,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : 4) void split_kernel(Sp
     for (int j = 0; j < 8; j++) x[j] = score[j >> 2][j & 3] * a.score_scale;
     int here = t.known ? last - base - v_key : 0;  // how many of the lane's keys there are
     bool whole = __all(here >= 8);
+    seen |= __ballot(here > 0);
     if (!whole) {
 #pragma unroll
       for (int j = 0; j < 8; j++) {
@@ -302,6 +304,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : 4) void split_kernel(Sp
     }
   }
 
+  if (seen) m = fmaxf(m, kLowest);
   // the four waves' sums
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
@@ -366,7 +369,7 @@ __global__ __launch_bounds__(kWaves * 64) void join_kernel(SplitArgs s) {
     float top = m;
 #pragma unroll
     for (int j = 0; j < kAhead; j++) top = fmaxf(top, stat[j][0]);
-    if (top == kMinusInf) continue;
+    if (top == kMinusInf) continue;  // chunks without keys
     float f = __builtin_amdgcn_exp2f(m - top);
     m = top, l *= f, o *= f;
 #pragma unroll

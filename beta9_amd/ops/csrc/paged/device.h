@@ -28,7 +28,10 @@ template <class C> struct Vec {
   typedef typename C::T x8 __attribute__((ext_vector_type(8)));
 };
 
+// A running maximum is -inf where no key has been seen, and at least kLowest where one has, also one whose score is NaN or
+// -inf: a maximum passes over NaN, and what was seen must not be taken for nothing when parts are joined.
 constexpr float kMinusInf = -__builtin_inff();
+constexpr float kLowest = -__FLT_MAX__;
 
 // Inclusive sums, the sum and the maximum over the lanes of whole numbers, by moves within the registers: about 50 cycles,
 // where exchanges through LDS take 130 for each of the six steps.

@@ -510,6 +510,46 @@ def test_values_that_are_not_finite_reach_the_rows_that_see_them(device, dim, ba
         assert ((got.cpu().double() - want).abs() <= off)[..., rest].all()
 
 
+# A row whose scores are not all numbers, in the operator's split and unsplit forms: `room` is the pages of 16 that a table
+# row has, which decides between them.
+NUMBERLESS = pytest.mark.parametrize("kind,cached,dim", [("bf16", "bf16", 64), ("fp16", "fp16", 128), ("bf16", "e4m3", 80), ("bf16", "bf16", 256)])
+
+
+@both
+@NUMBERLESS
+@pytest.mark.parametrize("lens,room", [([300, 0, 17, 300], 20), ([5000, 0, 17, 4100], 320), ([700] * 300, 44)])
+def test_a_query_that_is_no_number_in_decode(device, kind, cached, dim, lens, room):
+    """Its row is NaN, however its keys are split, and no other; without keys it is zero all the same."""
+    gen = torch.Generator().manual_seed(dim)
+    k_cache, v_cache, tables, scales = make_cache(gen, lens, 2, dim, 16, kind, cached, device)
+    cache = (k_cache, v_cache, [t + [0] * (room - len(t)) for t in tables], scales)
+    q = torch.randn((len(lens), 4, dim), generator=gen).to(TYPES[kind]).to(device)
+    want = run_decode(q, cache, lens)
+    bad = q.clone()
+    for r, head in ((0, 1), (1, 0), (2, 3)):
+        bad[r, head, dim // 2] = math.nan
+    got = run_decode(bad, cache, lens)
+    for r, head in ((0, 1), (1, 0), (2, 3)):
+        assert got[r, head].isnan().all() if lens[r] else (got[r, head] == 0).all()
+        got[r, head] = want[r, head]
+    assert torch.equal(got, want)
+
+
+@both
+@NUMBERLESS
+def test_a_stretch_of_keys_that_are_no_numbers_in_decode(device, kind, cached, dim):
+    """Whole chunks of it, the first, inner ones and the last: they make the heads that read them NaN."""
+    gen = torch.Generator().manual_seed(dim)
+    for first, last in ((0, 512), (1024, 2048), (4864, 5000)):
+        k_cache, v_cache, tables, scales = make_cache(gen, [5000], 2, dim, 16, kind, cached, device)
+        q = torch.randn((1, 4, dim), generator=gen).to(TYPES[kind]).to(device)
+        raw = torch.uint8 if cached == "e4m3" else torch.int16  # 0x7f..: NaN in each of the types
+        for t in range(first, last):
+            k_cache.view(raw)[tables[0][t // 16], 1, t % 16, dim - 1] = 0x7F if cached == "e4m3" else 0x7FFF
+        got = run_decode(q, (k_cache, v_cache, tables, scales), [5000])
+        assert got[:, 2:].isnan().all()
+        check_attention(got[:, :2], q[:, :2], (k_cache[:, :1], v_cache[:, :1], tables, scales), [5000], [0, 1])
+
 @both
 @pytest.mark.parametrize("dim", [80, 64, 128])
 def test_scores_far_apart(device, dim):
