@@ -515,6 +515,17 @@ def test_values_that_are_not_finite_reach_the_rows_that_see_them(device, dim, ba
 NUMBERLESS = pytest.mark.parametrize("kind,cached,dim", [("bf16", "bf16", 64), ("fp16", "fp16", 128), ("bf16", "e4m3", 80), ("bf16", "bf16", 256)])
 
 
+def check_all_but(got, q, cache, lens, cu, places):
+    """NaN at the places (row, head); the other rows are what they are beside a finite q, to what rounding allows. Their bits
+    may differ: the rows of a wave move their running maxima together, and so round probabilities at one scale or another."""
+    want, off = attention_oracle(q, *cache[:3], lens, cu, q.shape[-1] ** -0.5, *cache[3])
+    got = got.cpu().double()
+    for r, head in places:
+        assert got[r, head].isnan().all()
+        got[r, head] = want[r, head]
+    assert ((got - want).abs() <= off).all()
+
+
 @both
 @NUMBERLESS
 @pytest.mark.parametrize("lens,room", [([300, 0, 17, 300], 20), ([5000, 0, 17, 4100], 320), ([700] * 300, 44)])
@@ -524,15 +535,11 @@ def test_a_query_that_is_no_number_in_decode(device, kind, cached, dim, lens, ro
     k_cache, v_cache, tables, scales = make_cache(gen, lens, 2, dim, 16, kind, cached, device)
     cache = (k_cache, v_cache, [t + [0] * (room - len(t)) for t in tables], scales)
     q = torch.randn((len(lens), 4, dim), generator=gen).to(TYPES[kind]).to(device)
-    want = run_decode(q, cache, lens)
-    bad = q.clone()
-    for r, head in ((0, 1), (1, 0), (2, 3)):
+    bad, places = q.clone(), [(0, 1), (1, 0), (2, 3)]
+    for r, head in places:
         bad[r, head, dim // 2] = math.nan
     got = run_decode(bad, cache, lens)
-    for r, head in ((0, 1), (1, 0), (2, 3)):
-        assert got[r, head].isnan().all() if lens[r] else (got[r, head] == 0).all()
-        got[r, head] = want[r, head]
-    assert torch.equal(got, want)
+    check_all_but(got, q, cache, lens, list(range(len(lens) + 1)), [p for p in places if lens[p[0]]])
 
 
 @both
