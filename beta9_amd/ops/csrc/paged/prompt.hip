@@ -583,6 +583,17 @@ __global__ __launch_bounds__(kWaves * 64, waves_of(D, sizeof(typename C::T) == 1
   __syncthreads();
   if (again) pass(Constant<1>{});
 
+  // A row that the part's first key is not too late for, and that has no maximum, saw only scores of NaN or -inf, or only
+  // entries that name no page. Which of both is looked up here: in the pass it would cost registers.
+  if (__any(m == kMinusInf && position >= begin * kKeys)) {
+#pragma unroll 1
+    for (int tile = begin; tile < end; tile++) {
+      uint64_t present = present_of(entry_of(tile));
+      int count = position - tile * kKeys + 1;  // keys of the tile that are not past the row
+      if (count > 0 && (present << (64 - min(count, 64)))) m = fmaxf(m, kLowest);
+    }
+  }
+
   clear_rest();
   l += __shfl_xor(l, 32);
   if (w.parts > 1) {

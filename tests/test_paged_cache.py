@@ -558,6 +558,40 @@ def test_a_stretch_of_keys_that_are_no_numbers_in_decode(device, kind, cached, d
         check_attention(got[:, :2], q[:, :2], (k_cache[:, :1], v_cache[:, :1], tables, scales), [5000], [0, 1])
 
 @both
+@NUMBERLESS
+@pytest.mark.parametrize("new,held,room", [([40, 3], [100, 0], 12), ([7, 0, 3], [3000, 0, 900], 200), ([300, 300], [0, 700], 66)])
+def test_a_query_that_is_no_number_in_a_prompt(device, kind, cached, dim, new, held, room):
+    gen = torch.Generator().manual_seed(dim)
+    lens = [h + n for h, n in zip(held, new)]
+    cu = [0]
+    for n in new:
+        cu.append(cu[-1] + n)
+    k_cache, v_cache, tables, scales = make_cache(gen, lens, 2, dim, 16, kind, cached, device)
+    cache = (k_cache, v_cache, [t + [0] * (room - len(t)) for t in tables], scales)
+    q = torch.randn((cu[-1], 4, dim), generator=gen).to(TYPES[kind]).to(device)
+    bad = q.clone()
+    places = [(0, 1), (2, 3), (cu[-1] - 1, 0)]
+    for r, head in places:
+        bad[r, head, dim // 2] = math.nan
+    check_all_but(run_prompt(bad, cache, lens, cu), q, cache, lens, cu, places)
+
+
+@both
+@NUMBERLESS
+def test_a_newest_key_that_is_no_number_alone_in_its_part(device, kind, cached, dim):
+    """1025 keys are four parts of 256 and one of a single key, the row's own; 1030 with the last six tokens new."""
+    gen = torch.Generator().manual_seed(dim)
+    for n in (1, 6):
+        length = 1024 + n
+        k_cache, v_cache, tables, scales = make_cache(gen, [length], 2, dim, 16, kind, cached, device)
+        q = torch.randn((n, 4, dim), generator=gen).to(TYPES[kind]).to(device)
+        raw = torch.uint8 if cached == "e4m3" else torch.int16
+        k_cache.view(raw)[tables[0][1024 // 16], 1, 0, 0] = 0x7F if cached == "e4m3" else 0x7FFF
+        got = run_prompt(q, (k_cache, v_cache, tables, scales), [length], [0, n])
+        assert got[:, 2:].isnan().all()
+        check_attention(got[:, :2], q[:, :2], (k_cache[:, :1], v_cache[:, :1], tables, scales), [length], [0, n])
+
+@both
 @pytest.mark.parametrize("dim", [80, 64, 128])
 def test_scores_far_apart(device, dim):
     """Scores of thousands, all equal scores, and a maximum that comes first or last."""
