@@ -328,10 +328,10 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : 4) void split_kernel(Sp
   }
   if (share.count == 1) {
     typename X::T* out = (typename X::T*)a.out + share.request * a.out_row + (head0 + head) * a.out_head + dim;
-    float f = sum == 0.f ? 0.f : a.value_scale / sum;
+    float f = a.value_scale / sum;  // by zero where all scores were -inf: NaN, as the formula has it
 #pragma unroll
     for (int i = 0; i < K::kPer; i++)
-      if (!kPad || dim + i < a.dim) out[i] = (typename X::T)(sum == 0.f ? 0.f : o[i] * f);
+      if (!kPad || dim + i < a.dim) out[i] = (typename X::T)(top == kMinusInf ? 0.f : o[i] * f);
   } else {
     int64_t at = (int64_t)blockIdx.x * a.heads + head0 + head;
 #pragma unroll
@@ -393,9 +393,9 @@ __global__ __launch_bounds__(kWaves * 64) void join_kernel(SplitArgs s) {
     l += f * l_lds[w][here], o += f * *reinterpret_cast<const f32x4*>(&o_lds[w][here][dim]);
   }
   typename X::T* out = (typename X::T*)a.out + share.request * a.out_row + head * a.out_head + dim;
-  f = l == 0.f ? 0.f : a.value_scale / l;
+  f = a.value_scale / l;
 #pragma unroll
-  for (int i = 0; i < 4; i++) out[i] = (typename X::T)(l == 0.f ? 0.f : o[i] * f);
+  for (int i = 0; i < 4; i++) out[i] = (typename X::T)(top == kMinusInf ? 0.f : o[i] * f);
 }
 
 // Keys of a chunk at least: shorter ones spend their time on starting and joining.

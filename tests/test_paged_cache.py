@@ -591,6 +591,39 @@ def test_a_newest_key_that_is_no_number_alone_in_its_part(device, kind, cached, 
         assert got[:, 2:].isnan().all()
         check_attention(got[:, :2], q[:, :2], (k_cache[:, :1], v_cache[:, :1], tables, scales), [length], [0, n])
 
+def infinite_keys(gen, lens, dim, kind, device, room, where=lambda t: True):
+    """A cache of two kv heads; the keys t of the first that `where` names hold inf in dim 7, so that a query negative there
+    has the score -inf."""
+    k_cache, v_cache, tables, scales = make_cache(gen, lens, 2, dim, 16, kind, kind, device)
+    for r, n in enumerate(lens):
+        t = torch.tensor([t for t in range(n) if where(t)], dtype=torch.int64)
+        if len(t):
+            k_cache[torch.tensor(tables[r], dtype=torch.int64)[t // 16].to(device), 0, (t % 16).to(device), 7] = math.inf
+    return k_cache, v_cache, [t + [0] * (room - len(t)) for t in tables], scales
+
+
+@both
+@pytest.mark.parametrize("kind,dim", [("bf16", 64), ("fp16", 128), ("bf16", 80), ("fp16", 256)])
+@pytest.mark.parametrize("lens,room", [([1, 0, 40, 300], 20), ([1, 0, 700, 5000], 320)])
+def test_scores_of_minus_infinity_in_decode(device, kind, dim, lens, room):
+    """Where all that a row sees have it, the softmax is 0 / 0: NaN. Where some have, they weigh nothing."""
+    gen = torch.Generator().manual_seed(dim)
+    q = torch.randn((4, 4, dim), generator=gen).to(TYPES[kind]).to(device)
+    q[:, :2, 7] = -1.0
+    cache = infinite_keys(gen, lens, dim, kind, device, room)
+    got = run_decode(q, cache, lens)
+    assert got[[0, 2, 3], :2].isnan().all() and (got[1] == 0).all()
+    check_attention(got[:, 2:], q[:, 2:], (cache[0][:, 1:], cache[1][:, 1:], *cache[2:]), lens, [0, 1, 2, 3, 4])
+    # the same as if those keys were absent: pages 0 and 4 to 19 of each row
+    gone = lambda t: t // 16 == 0 or 4 <= t // 16 < 20  # noqa: E731
+    cache = infinite_keys(gen, lens, dim, kind, device, room, gone)
+    got = run_decode(q, cache, lens)
+    left = [[-1 if gone(16 * i) else p for i, p in enumerate(t)] for t in cache[2]]
+    some = [r for r, n in enumerate(lens) if any(not gone(t) for t in range(n))]
+    want = [lens[r] for r in some]
+    cache = (cache[0][:, :1], cache[1][:, :1], [left[r] for r in some], cache[3])
+    check_attention(got[some, :2], q[some, :2], cache, want, list(range(len(some) + 1)))
+
 @both
 @pytest.mark.parametrize("dim", [80, 64, 128])
 def test_scores_far_apart(device, dim):
