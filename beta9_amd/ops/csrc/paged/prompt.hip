@@ -606,7 +606,7 @@ __global__ __launch_bounds__(kWaves * 64, waves_of(D, sizeof(typename C::T) == 1
         *reinterpret_cast<f32x4*>(s.part + at * D + 4 * half + 32 * d + 2 * r) = f32x4{acc[d][r], acc[d][r + 1], acc[d][r + 2], acc[d][r + 3]};
     return;
   }
-  float f = l == 0.f ? 0.f : a.value_scale / l;
+  float f = a.value_scale / l;  // by zero where all scores were -inf: NaN, as the formula has it
   // Through the wave's part of LDS, so that each store fills whole lines: with 16 bytes of 32 rows a store, the results of a
   // workgroup (head dim 128) took 2 us and more. Chunks are exchanged by the row as for K.
   char* mine = lds + wave * 32 * kRowBytes;
@@ -616,7 +616,7 @@ __global__ __launch_bounds__(kWaves * 64, waves_of(D, sizeof(typename C::T) == 1
     for (int r = 0; r < 16; r += 4) {
       typename Vec<X>::x4 y;
 #pragma unroll
-      for (int i = 0; i < 4; i++) y[i] = (Out)(l == 0.f ? 0.f : acc[d][r + i] * f);
+      for (int i = 0; i < 4; i++) y[i] = (Out)(m == kMinusInf ? 0.f : acc[d][r + i] * f);
       *reinterpret_cast<typename Vec<X>::x4*>(mine + n * kRowBytes + (((4 * d + r / 4) ^ (n & (kChunks - 1))) * 16) + 8 * half) = y;
     }
   int place = real ? (w.row0 + token) * a.heads + head : -1;  // fits: rows by heads do; `out` has no gaps
@@ -661,10 +661,10 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs s) {
   }
   int token = s.by_group.divide(row), head = kv_head * s.group + row - token * s.group;
   typename X::T* out = (typename X::T*)a.out + (w.row0 + token) * a.out_row + head * a.out_head + dim;
-  float f = l == 0.f ? 0.f : a.value_scale / l;
+  float f = a.value_scale / l;
   typename Vec<X>::x4 y;
 #pragma unroll
-  for (int i = 0; i < 4; i++) y[i] = (typename X::T)(l == 0.f ? 0.f : o[i] * f);
+  for (int i = 0; i < 4; i++) y[i] = (typename X::T)(m == kMinusInf ? 0.f : o[i] * f);
   *reinterpret_cast<typename Vec<X>::x4*>(out) = y;
 }
 

@@ -176,7 +176,8 @@ def decode_attention(
     [B, heads, head dim], row r over the first kv_lens[r] tokens of request
     r. heads is a multiple of the cache's; head h reads kv head
     h // (heads // kv heads). scale is 1 / sqrt(head dim) if not given. A
-    row with no tokens gives zeros. ``out`` (contiguous) is written if
+    row with no tokens gives zeros; scores that are NaN, or all -inf, give
+    NaN, however the keys are split. ``out`` (contiguous) is written if
     given."""
     scale = q.shape[-1] ** -0.5 if scale is None else scale
     ext = _native(q)
@@ -201,7 +202,8 @@ def prompt_attention(
     r's rows cu_new[r] .. cu_new[r + 1] - 1 are its last tokens among its
     kv_lens[r], which the cache holds already (``write_kv`` comes first).
     The j-th of n new rows sees the first kv_lens[r] - n + j + 1 tokens; a
-    row that sees none gives zeros. Rows behind the last request are zero in
+    row that sees none gives zeros, one whose scores are NaN or all -inf NaN.
+    Rows behind the last request are zero in
     a new result, and left as they are in ``out`` (contiguous)."""
     scale = q.shape[-1] ** -0.5 if scale is None else scale
     ext = _native(q)

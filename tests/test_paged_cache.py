@@ -625,6 +625,29 @@ def test_scores_of_minus_infinity_in_decode(device, kind, dim, lens, room):
     check_attention(got[some, :2], q[some, :2], cache, want, list(range(len(some) + 1)))
 
 @both
+@pytest.mark.parametrize("kind,dim", [("bf16", 64), ("fp16", 128), ("bf16", 80), ("fp16", 256)])
+@pytest.mark.parametrize("length,rows,room", [(90, 90, 8), (90, 100, 8), (3000, 5, 200)])
+def test_scores_of_minus_infinity_in_a_prompt(device, kind, dim, length, rows, room):
+    """The same, and rows that see no key stay zero."""
+    gen = torch.Generator().manual_seed(dim)
+    q = torch.randn((rows, 4, dim), generator=gen).to(TYPES[kind]).to(device)
+    q[:, :2, 7] = -1.0
+    none = max(0, rows - length)
+    cache = infinite_keys(gen, [length], dim, kind, device, room)
+    got = run_prompt(q, cache, [length], [0, rows])
+    assert (got[:none] == 0).all() and got[none:, :2].isnan().all()
+    check_attention(got[:, 2:], q[:, 2:], (cache[0][:, 1:], cache[1][:, 1:], *cache[2:]), [length], [0, rows])
+    # the first three pages and a later stretch: as if those keys were absent
+    gone = lambda t: t < 48 or 512 <= t < 1104  # noqa: E731
+    cache = infinite_keys(gen, [length], dim, kind, device, room, gone)
+    got = run_prompt(q, cache, [length], [0, rows])
+    first = none + 48 if rows >= length else 0  # the first row that sees another
+    assert (got[:none] == 0).all() and got[none:first, :2].isnan().all()
+    left = [[-1 if gone(16 * i) else p for i, p in enumerate(cache[2][0])]]
+    check_attention(got[first:, :2], q[first:, :2], (cache[0][:, :1], cache[1][:, :1], left, cache[3]), [length], [0, rows - first])
+
+
+@both
 @pytest.mark.parametrize("dim", [80, 64, 128])
 def test_scores_far_apart(device, dim):
     """Scores of thousands, all equal scores, and a maximum that comes first or last."""
