@@ -13,6 +13,7 @@ through its AttentionInterface: the new keys and values go into the pages
 
 from __future__ import annotations
 
+import math
 import threading
 from typing import Any, List, Optional
 
@@ -51,6 +52,20 @@ def register() -> str:
     AttentionInterface.register(NAME, attention)
     AttentionMaskInterface.register(NAME, lambda *args, **kwargs: None)  # lengths and positions say it all
     return NAME
+
+
+def sample(logits, temperature: float) -> Optional[int]:
+    """A token at a temperature above zero; None if the largest logit is not
+    a finite number."""
+    import torch
+
+    top = logits.max()
+    if not math.isfinite(top.item()):
+        return None
+    # The largest is taken off first, and the temperature kept in range: the quotients then pass 32 bits only towards -inf,
+    # whose weight is 0, and a temperature next to zero takes the largest.
+    t = min(max(temperature, 2.0**-100), 2.0**100)
+    return int(torch.multinomial(torch.softmax((logits - top) / t, dim=-1), 1).item())
 
 
 class PagedDecoder:
@@ -126,8 +141,9 @@ class PagedDecoder:
             started.append(row)
         return started
 
-    def _forward(self, rows: List[int], ids: List[int], new: List[int], decode: bool) -> List[int]:
-        """One pass over the packed tokens of `rows`; each row's next token."""
+    def _forward(self, rows: List[int], ids: List[int], new: List[int], decode: bool) -> List[Optional[int]]:
+        """One pass over the packed tokens of `rows`; each row's next token,
+        None where its logits give none."""
         import torch
 
         put = lambda x, t: torch.tensor(x, dtype=t, device=self.device)  # noqa: E731
@@ -149,15 +165,18 @@ class PagedDecoder:
         for i, row in enumerate(rows):
             t = self.rows[row].temperature
             if t > 0:
-                tokens[i] = int(torch.multinomial(torch.softmax(logits[i] / t, dim=-1), 1).item())
+                tokens[i] = sample(logits[i], t)
         return tokens
 
-    def _take(self, rows: List[int], tokens: List[int]) -> None:
+    def _take(self, rows: List[int], tokens: List[Optional[int]]) -> None:
         for row, token in zip(rows, tokens):
             req = self.rows[row]
-            req.out_ids.append(token)
+            if token is None:
+                req.error = ValueError("no token can be drawn: the model's logits are not finite")
+            else:
+                req.out_ids.append(token)
             full = self.lens[row] >= self.args.max_model_len
-            if (self.eos_id is not None and token == self.eos_id) or len(req.out_ids) >= req.max_tokens or full:
+            if token is None or (self.eos_id is not None and token == self.eos_id) or len(req.out_ids) >= req.max_tokens or full:
                 self._ended.append(req)
                 self.rows[row] = None
                 self._freed.append(row)

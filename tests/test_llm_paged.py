@@ -157,3 +157,47 @@ def test_paged_on_the_gpu(kind, heads):
         # times a few 2^-8, e4m3 keys and values by 2^-4 of theirs; a wrong row or page moves them by the whole spread
         off = {"paged": 0.25, "paged_e4m3": 0.75}[kind]
         assert float(logits.max() - logits[tokens[0]]) <= off * float(logits.std())
+
+
+def together(engine, requests):
+    """generate() of (prompt, max_tokens, temperature) at once; each one's text or exception."""
+
+    async def main():
+        calls = [engine.generate(*r) for r in requests]
+        try:
+            return await asyncio.wait_for(asyncio.gather(*calls, return_exceptions=True), 120)
+        finally:
+            await engine.stop()
+
+    return asyncio.run(main())
+
+
+@pytest.mark.parametrize("temperature", [1e-40, 1e-300, 5e-324])
+def test_a_temperature_next_to_zero_is_greedy_and_leaves_the_others_alone(temperature):
+    want = together(LLMEngine(args(kv_cache="paged")), [("hello", 8, 0.0), ("bad", 8, 0.0)])
+    got = together(LLMEngine(args(kv_cache="paged")), [("hello", 8, 0.0), ("bad", 8, temperature)])
+    assert got == want
+
+
+def test_a_temperature_without_bound_runs():
+    got = together(LLMEngine(args(kv_cache="paged")), [("hello", 8, 1e300), ("there", 8, float("inf")), ("x", 3, float("nan"))])
+    assert all(isinstance(t, str) for t in got)
+
+
+def test_logits_that_are_no_numbers_end_their_own_request_only():
+    want = together(LLMEngine(args(kv_cache="paged")), [("hello", 8, 0.0)])
+    engine = LLMEngine(args(kv_cache="paged"))
+    forward, calls = engine.model.forward, []
+
+    def planted(*a, **more):
+        out = forward(*a, **more)
+        calls.append(out.logits.shape[1])
+        if len(calls) == 3:  # a decode step of both requests: the second one's
+            out.logits[0, 1, 7] = float("nan")
+        return out
+
+    engine.model.forward = planted
+    got = together(engine, [("hello", 8, 0.0), ("there", 8, 0.5)])
+    assert calls[2] == 2 and got[:1] == want
+    assert isinstance(got[1], ValueError) and "finite" in str(got[1])
+    assert engine.paged.cache.free_count.tolist() == [engine.paged.cache.pages]
