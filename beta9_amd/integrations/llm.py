@@ -161,15 +161,16 @@ class LLMEngine:
 
     async def _loop_paged(self) -> None:
         while True:
-            arrived = [] if self.paged.active else [await self._queue.get()]
+            idle = not self.paged.active
+            for r in self.paged.take_ended():
+                r.done.set()
+            arrived = [await self._queue.get()] if idle else []
             while not self._queue.empty():
                 arrived.append(self._queue.get_nowait())
             try:
-                ended = await asyncio.get_event_loop().run_in_executor(None, self.paged.step, arrived)
+                await asyncio.get_event_loop().run_in_executor(None, self.paged.step, arrived)
             except Exception as e:
-                ended = self.paged.fail(e)
-            for r in ended:
-                r.done.set()
+                self.paged.fail(e)
 
     def _decode_group(self, batch: List[_Request]) -> None:
         """One step-group: batched greedy/sampling decode with KV cache;

@@ -15,7 +15,8 @@ from __future__ import annotations
 
 import math
 import threading
-from typing import Any, List, Optional
+from collections import deque
+from typing import Any, Deque, List, Optional
 
 NAME = "beta9_paged"
 KINDS = ("dense", "paged", "paged_e4m3")
@@ -102,14 +103,23 @@ class PagedDecoder:
         self.lens = [0] * args.max_num_seqs  # tokens held, as the GPU has them
         self.reserved = [0] * args.max_num_seqs  # pages a row may come to hold
         self.waiting: List[Any] = []
-        self._ended: List[Any] = []
+        # A step whose loop was stopped runs on in its thread; the next one waits for it. What it ends stays here until a loop
+        # takes it. Requests go from `waiting` to `rows` to `_ended`, and are entered in the next before they leave the last,
+        # so that a loop that looks at the three in this order beside a running step misses none.
+        self._ended: Deque[Any] = deque()
         self._freed: List[int] = []
-        # a step whose loop was stopped runs on in its thread; the next one waits for it
         self._lock = threading.Lock()
 
     @property
     def active(self) -> bool:
-        return any(r is not None for r in self.rows) or bool(self.waiting)
+        return bool(self.waiting) or any(r is not None for r in self.rows)
+
+    def take_ended(self) -> List[Any]:
+        """The requests that ended since the last call."""
+        ended = []
+        while self._ended:
+            ended.append(self._ended.popleft())
+        return ended
 
     def _most(self, req) -> int:
         """Tokens the request can come to hold: its last one is never written."""
@@ -123,7 +133,8 @@ class PagedDecoder:
             if req.max_tokens <= 0 or not req.prompt_ids:
                 if not req.prompt_ids:
                     req.error = ValueError("the prompt has no tokens")
-                self._ended.append(self.waiting.pop(0))
+                self._ended.append(req)
+                self.waiting.pop(0)
                 continue
             pages = self.cache.pages_for(self._most(req))
             if len(req.prompt_ids) > self.args.max_model_len or pages > self.cache.pages:
@@ -131,13 +142,15 @@ class PagedDecoder:
                     f"a request of {len(req.prompt_ids)} + {req.max_tokens} tokens does not fit the cache: "
                     f"{self.args.max_model_len} tokens a row, {self.cache.pages} pages of {self.cache.page_size}"
                 )
-                self._ended.append(self.waiting.pop(0))
+                self._ended.append(req)
+                self.waiting.pop(0)
                 continue
             free = [r for r, q in enumerate(self.rows) if q is None]
             if not free or sum(self.reserved) + pages > self.cache.pages:
                 break  # first come, first served
             row = free[0]
-            self.rows[row], self.reserved[row], self.lens[row] = self.waiting.pop(0), pages, 0
+            self.rows[row], self.reserved[row], self.lens[row] = req, pages, 0
+            self.waiting.pop(0)
             started.append(row)
         return started
 
@@ -181,34 +194,32 @@ class PagedDecoder:
                 self.rows[row] = None
                 self._freed.append(row)
 
-    def fail(self, error: Exception) -> List[Any]:
+    def fail(self, error: Exception) -> None:
         with self._lock:
-            return self._fail(error)
+            self._fail(error)
 
-    def _fail(self, error: Exception) -> List[Any]:
+    def _fail(self, error: Exception) -> None:
         """After a step that raised: ends every request with its error, and
         starts again with an empty cache."""
         import torch
 
-        ended = [r for r in self.rows if r is not None] + self.waiting
-        for req in ended:
+        for req in [r for r in self.rows if r is not None] + self.waiting:
             req.error = error
-        ended = ended + [r for r in self._ended if r not in ended]
+            self._ended.append(req)
         n = len(self.rows)
         self.rows, self.lens, self.reserved, self.waiting = [None] * n, [0] * n, [0] * n, []
         self.cache.release(torch.ones(n, dtype=torch.bool, device=self.device))
-        return ended
 
-    def step(self, arrived: List[Any]) -> List[Any]:
+    def step(self, arrived: List[Any]) -> None:
         """Takes in what arrived, reads the prompts that fit, decodes one
-        token of every active request; returns the requests that ended."""
+        token of every active request."""
         with self._lock:
-            return self._step(arrived)
+            self._step(arrived)
 
-    def _step(self, arrived: List[Any]) -> List[Any]:
+    def _step(self, arrived: List[Any]) -> None:
         import torch
 
-        self._ended, self._freed = [], []
+        self._freed = []
         self.waiting.extend(arrived)
         with torch.inference_mode():
             started = self._admit()
@@ -226,4 +237,3 @@ class PagedDecoder:
                 self.cache.release(done.to(self.device))
                 for row in self._freed:
                     self.reserved[row] = self.lens[row] = 0
-        return self._ended

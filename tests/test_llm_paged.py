@@ -1,6 +1,7 @@
 """The LLM engine over the paged key-value cache."""
 
 import asyncio
+import threading
 
 import pytest
 
@@ -201,3 +202,51 @@ def test_logits_that_are_no_numbers_end_their_own_request_only():
     assert calls[2] == 2 and got[:1] == want
     assert isinstance(got[1], ValueError) and "finite" in str(got[1])
     assert engine.paged.cache.free_count.tolist() == [engine.paged.cache.pages]
+
+
+class Held:
+    """The engine's forward passes wait, from the first one on, until they are let go."""
+
+    def __init__(self, engine):
+        self.entered, self.go, forward = threading.Event(), threading.Event(), engine.paged._forward
+
+        def wait(*a):
+            self.entered.set()
+            assert self.go.wait(60)
+            return forward(*a)
+
+        engine.paged._forward = wait
+
+
+@pytest.mark.parametrize("another", [True, False])
+def test_a_request_that_ends_in_a_step_whose_loop_was_stopped(another):
+    """It is answered when the engine runs again, with another request or without one, in that step or after it."""
+    for early in (False, True):
+        engine = LLMEngine(args(kv_cache="paged"))
+        held = Held(engine)
+
+        async def main():
+            in_thread = asyncio.get_event_loop().run_in_executor
+            first = asyncio.create_task(engine.generate("hello", 1))
+            assert await in_thread(None, held.entered.wait, 60)
+            await engine.stop()
+            if not early:
+                held.go.set()
+                while engine.paged.active:
+                    await asyncio.sleep(0.01)
+            if another:
+                second = asyncio.create_task(engine.generate("there", 2))
+                await asyncio.sleep(0)
+            else:
+                await engine.start()
+            await asyncio.sleep(0.05)
+            held.go.set()
+            try:
+                got = [await asyncio.wait_for(first, 30)]
+                return got + ([await asyncio.wait_for(second, 30)] if another else [])
+            finally:
+                await engine.stop()
+
+        got = asyncio.run(main())
+        want = together(LLMEngine(args(kv_cache="paged")), [("hello", 1, 0.0), ("there", 2, 0.0)])
+        assert got == want[: len(got)]
