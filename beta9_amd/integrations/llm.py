@@ -164,11 +164,12 @@ class LLMEngine:
             idle = not self.paged.active
             for r in self.paged.take_ended():
                 r.done.set()
-            arrived = [await self._queue.get()] if idle else []
+            if idle:
+                self.paged.submit(await self._queue.get())
             while not self._queue.empty():
-                arrived.append(self._queue.get_nowait())
+                self.paged.submit(self._queue.get_nowait())
             try:
-                await asyncio.get_event_loop().run_in_executor(None, self.paged.step, arrived)
+                await asyncio.get_event_loop().run_in_executor(None, self.paged.step)
             except Exception as e:
                 self.paged.fail(e)
 

@@ -114,6 +114,10 @@ class PagedDecoder:
     def active(self) -> bool:
         return bool(self.waiting) or any(r is not None for r in self.rows)
 
+    def submit(self, req) -> None:
+        """A request for the next step."""
+        self.waiting.append(req)
+
     def take_ended(self) -> List[Any]:
         """The requests that ended since the last call."""
         ended = []
@@ -194,6 +198,10 @@ class PagedDecoder:
                 self.rows[row] = None
                 self._freed.append(row)
 
+    def _end(self, req, error: Exception) -> None:
+        req.error = error
+        self._ended.append(req)
+
     def fail(self, error: Exception) -> None:
         with self._lock:
             self._fail(error)
@@ -203,24 +211,27 @@ class PagedDecoder:
         starts again with an empty cache."""
         import torch
 
-        for req in [r for r in self.rows if r is not None] + self.waiting:
-            req.error = error
-            self._ended.append(req)
+        for row, req in enumerate(self.rows):
+            if req is not None:
+                self._end(req, error)
+                self.rows[row] = None
+        while self.waiting:
+            self._end(self.waiting[0], error)
+            self.waiting.pop(0)
         n = len(self.rows)
-        self.rows, self.lens, self.reserved, self.waiting = [None] * n, [0] * n, [0] * n, []
+        self.lens, self.reserved = [0] * n, [0] * n
         self.cache.release(torch.ones(n, dtype=torch.bool, device=self.device))
 
-    def step(self, arrived: List[Any]) -> None:
-        """Takes in what arrived, reads the prompts that fit, decodes one
-        token of every active request."""
+    def step(self) -> None:
+        """Reads the waiting prompts that fit, decodes one token of every
+        active request."""
         with self._lock:
-            self._step(arrived)
+            self._step()
 
-    def _step(self, arrived: List[Any]) -> None:
+    def _step(self) -> None:
         import torch
 
         self._freed = []
-        self.waiting.extend(arrived)
         with torch.inference_mode():
             started = self._admit()
             if started:

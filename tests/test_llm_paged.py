@@ -2,6 +2,7 @@
 
 import asyncio
 import threading
+from concurrent.futures import ThreadPoolExecutor
 
 import pytest
 
@@ -250,3 +251,33 @@ def test_a_request_that_ends_in_a_step_whose_loop_was_stopped(another):
         got = asyncio.run(main())
         want = together(LLMEngine(args(kv_cache="paged")), [("hello", 1, 0.0), ("there", 2, 0.0)])
         assert got == want[: len(got)]
+
+
+def test_a_request_whose_step_was_stopped_before_it_began():
+    """The step waits for a thread when the loop is stopped, and never runs; its request is not lost with it."""
+    engine = LLMEngine(args(kv_cache="paged"))
+    busy, go = threading.Event(), threading.Event()
+
+    def hold():
+        busy.set()
+        assert go.wait(60)
+
+    async def main():
+        loop = asyncio.get_event_loop()
+        loop.set_default_executor(ThreadPoolExecutor(1))
+        other = loop.run_in_executor(None, hold)
+        while not busy.is_set():
+            await asyncio.sleep(0.01)
+        first = asyncio.create_task(engine.generate("hello", 3))
+        await asyncio.sleep(0.05)
+        await engine.stop()
+        go.set()
+        await other
+        second = asyncio.create_task(engine.generate("there", 2))
+        try:
+            return [await asyncio.wait_for(t, 30) for t in (second, first)]
+        finally:
+            await engine.stop()
+
+    want = together(LLMEngine(args(kv_cache="paged")), [("there", 2, 0.0), ("hello", 3, 0.0)])
+    assert asyncio.run(main()) == want
