@@ -168,10 +168,7 @@ class LLMEngine:
                 self.paged.submit(await self._queue.get())
             while not self._queue.empty():
                 self.paged.submit(self._queue.get_nowait())
-            try:
-                await asyncio.get_event_loop().run_in_executor(None, self.paged.step)
-            except Exception as e:
-                self.paged.fail(e)
+            await asyncio.get_event_loop().run_in_executor(None, self.paged.step)
 
     def _decode_group(self, batch: List[_Request]) -> None:
         """One step-group: batched greedy/sampling decode with KV cache;

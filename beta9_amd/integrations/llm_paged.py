@@ -109,6 +109,7 @@ class PagedDecoder:
         self._ended: Deque[Any] = deque()
         self._freed: List[int] = []
         self._lock = threading.Lock()
+        self.broken: Optional[Exception] = None  # why no step can be run any more
 
     @property
     def active(self) -> bool:
@@ -202,13 +203,10 @@ class PagedDecoder:
         req.error = error
         self._ended.append(req)
 
-    def fail(self, error: Exception) -> None:
-        with self._lock:
-            self._fail(error)
-
     def _fail(self, error: Exception) -> None:
         """After a step that raised: ends every request with its error, and
-        starts again with an empty cache."""
+        starts again with an empty cache. If that raises too, the requests
+        of all later steps end with an error."""
         import torch
 
         for row, req in enumerate(self.rows):
@@ -220,13 +218,22 @@ class PagedDecoder:
             self.waiting.pop(0)
         n = len(self.rows)
         self.lens, self.reserved = [0] * n, [0] * n
-        self.cache.release(torch.ones(n, dtype=torch.bool, device=self.device))
+        if self.broken is None:
+            try:
+                self.cache.release(torch.ones(n, dtype=torch.bool, device=self.device))
+            except Exception as e:
+                self.broken = RuntimeError(f"the paged cache could not be reset after an error: {e}")
 
     def step(self) -> None:
         """Reads the waiting prompts that fit, decodes one token of every
-        active request."""
+        active request. An error ends the requests and is not raised."""
         with self._lock:
-            self._step()
+            try:
+                if self.broken is not None:
+                    raise self.broken
+                self._step()
+            except Exception as e:
+                self._fail(e)
 
     def _step(self) -> None:
         import torch

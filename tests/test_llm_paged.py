@@ -281,3 +281,18 @@ def test_a_request_whose_step_was_stopped_before_it_began():
 
     want = together(LLMEngine(args(kv_cache="paged")), [("there", 2, 0.0), ("hello", 3, 0.0)])
     assert asyncio.run(main()) == want
+
+
+def test_a_cache_that_cannot_be_reset_ends_every_request():
+    """As after a device error, which the release meets again: those in flight, those that wait, and all later ones."""
+    engine = LLMEngine(args(kv_cache="paged", max_num_seqs=2))
+
+    def planted(*a):
+        raise RuntimeError("planned")
+
+    engine.paged._forward = engine.paged.cache.release = planted
+    got = together(engine, [("hello", 3, 0.0), ("there", 3, 0.0), ("waits", 3, 0.0)])
+    assert [type(e) for e in got] == [RuntimeError] * 3 and not engine.paged.active
+    engine._queue = asyncio.Queue()
+    got = together(engine, [("later", 3, 0.0)])
+    assert isinstance(got[0], RuntimeError) and "reset" in str(got[0])
