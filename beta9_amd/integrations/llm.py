@@ -127,7 +127,7 @@ class LLMEngine:
             self.paged = PagedDecoder(self.model, self.args, self.eos_id, self.dtype, self.device)
 
     async def start(self) -> None:
-        if self._task is None:
+        if self._task is None or self._task.done():
             self._task = asyncio.create_task(self._loop() if self.paged is None else self._loop_paged())
 
     async def stop(self) -> None:

@@ -296,3 +296,20 @@ def test_a_cache_that_cannot_be_reset_ends_every_request():
     engine._queue = asyncio.Queue()
     got = together(engine, [("later", 3, 0.0)])
     assert isinstance(got[0], RuntimeError) and "reset" in str(got[0])
+
+
+@pytest.mark.parametrize("kind", ["dense", "paged"])
+def test_a_loop_that_has_finished_is_begun_again(kind):
+    engine = LLMEngine(args(kv_cache=kind))
+
+    async def main():
+        first = await engine.generate("hello", 2)
+        engine._task.cancel()
+        await asyncio.wait([engine._task])
+        try:
+            return first, await asyncio.wait_for(engine.generate("hello", 2), 30)
+        finally:
+            await engine.stop()
+
+    first, second = asyncio.run(main())
+    assert first == second
