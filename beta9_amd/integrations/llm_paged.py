@@ -87,6 +87,15 @@ class PagedDecoder:
                 f"kv_cache={args.kv_cache!r} needs full attention in every layer and a head dim that is a "
                 f"multiple of 8 up to {MAX_HEAD_DIM}; this model has {sorted(kinds)} and {dim}"
             )
+        # without layer types, a window is that of every layer
+        for name, set_to in (
+            ("sliding_window", None if getattr(cfg, "layer_types", None) else getattr(cfg, "sliding_window", None)),
+            ("attn_logit_softcapping", getattr(cfg, "attn_logit_softcapping", None)),
+        ):
+            if set_to is not None:
+                raise ValueError(
+                    f"kv_cache={args.kv_cache!r} serves attention without windows or caps; this model has {name} = {set_to}"
+                )
         if device != "cpu" and dtype not in (torch.bfloat16, torch.float16):
             raise ValueError(f"kv_cache={args.kv_cache!r} needs dtype='bfloat16' on a GPU, not {args.dtype!r}")
         model.set_attn_implementation(register())

@@ -313,3 +313,40 @@ def test_a_loop_that_has_finished_is_begun_again(kind):
 
     first, second = asyncio.run(main())
     assert first == second
+
+
+def test_models_that_need_more_than_full_attention_are_refused_when_built():
+    """A window for all layers is no layer type, and a cap on the scores neither: both came out at the first request."""
+    from transformers import Gemma2Config, Gemma2ForCausalLM, MistralConfig, MistralForCausalLM
+
+    from beta9_amd.integrations.llm_paged import PagedDecoder
+
+    sizes = dict(
+        vocab_size=300, hidden_size=64, intermediate_size=128, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2,
+        head_dim=16, max_position_embeddings=128,
+    )
+    build = lambda model: PagedDecoder(model.eval(), args(kv_cache="paged"), None, torch.float32, "cpu")  # noqa: E731
+    with pytest.raises(ValueError, match="sliding_window"):
+        build(MistralForCausalLM(MistralConfig(sliding_window=32, **sizes)))
+    full = dict(layer_types=["full_attention"] * 2, **sizes)
+    with pytest.raises(ValueError, match="softcapping"):
+        build(Gemma2ForCausalLM(Gemma2Config(attn_logit_softcapping=30.0, **full)))
+    # without a window and a cap they are served
+    for model in (
+        MistralForCausalLM(MistralConfig(sliding_window=None, **sizes)),
+        Gemma2ForCausalLM(Gemma2Config(attn_logit_softcapping=None, query_pre_attn_scalar=16, **full)),
+    ):
+        decoder, req = build(model), _Request([5, 6, 7], 4, 0.0)
+        decoder.submit(req)
+        while decoder.active:
+            decoder.step()
+        assert decoder.take_ended() == [req] and req.error is None
+        ids = [5, 6, 7]
+        model.set_attn_implementation("eager")
+        with torch.inference_mode():
+            for token in req.out_ids:
+                logits = model(input_ids=torch.tensor([ids]), use_cache=False).logits[0, -1]
+                # the same sums in another order: about 20 one after the other, of at most 128 terms, each off by 2^-24 a term
+                assert float(logits.max() - logits[token]) <= 1e-3 * float(logits.std())
+                ids.append(token)
+        assert len(req.out_ids) == 4
