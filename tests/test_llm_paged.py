@@ -350,3 +350,48 @@ def test_models_that_need_more_than_full_attention_are_refused_when_built():
                 assert float(logits.max() - logits[token]) <= 1e-3 * float(logits.std())
                 ids.append(token)
         assert len(req.out_ids) == 4
+
+
+@pytest.mark.gpu
+@pytest.mark.skipif(not torch.cuda.is_available(), reason="needs MI355X")
+@pytest.mark.parametrize("kind", ["paged", "paged_e4m3"])
+@pytest.mark.parametrize("heads", [4, 2])
+def test_every_token_of_the_paged_engine_on_the_gpu(kind, heads):
+    """Each token, those of the decode steps too, is within rounding of the best one in 64 bits behind the tokens before it."""
+    more = dict(hidden_size=256, intermediate_size=512, num_attention_heads=heads, kv_page_size=32)
+    engine = LLMEngine(args(kv_cache=kind, **more))
+    engine.eos_id = engine.paged.eos_id = None
+    got, errors = ids_of(engine, PROMPTS, STEPS)
+    assert errors == [None] * len(PROMPTS) and [len(t) for t in got] == STEPS
+    model = LLMEngine(args(**more)).model.double()
+    model.set_attn_implementation("eager")
+    # as for the first token: two layers' 2 x 7 products and 4 sums round to bf16, and with them each key and value that the
+    # cache holds, in e4m3 to 2^-4; a wrong row, page or position moves logits by their whole spread
+    off = {"paged": 0.25, "paged_e4m3": 0.75}[kind]
+    for prompt, tokens in zip(PROMPTS, got):
+        ids = engine.tokenizer.encode(prompt)
+        with torch.inference_mode():
+            whole = torch.tensor([ids + tokens[:-1]], device="cuda")
+            logits = model(input_ids=whole, use_cache=False).logits[0, len(ids) - 1 :]
+        far = logits.max(-1).values - logits.gather(1, torch.tensor(tokens, device="cuda")[:, None])[:, 0]
+        assert (far <= off * logits.std(-1)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.skipif(not torch.cuda.is_available(), reason="needs MI355X")
+def test_sampling_on_the_gpu():
+    """Temperatures of any size beside each other, and logits that are no numbers."""
+    engine = LLMEngine(args(kv_cache="paged"))
+    got = together(engine, [(p, 6, t) for p, t in zip(PROMPTS, (1e-40, 0.8, 1e300, float("inf"), 0.0, 1e-300))])
+    assert all(isinstance(t, str) for t in got)
+    engine._queue, forward = asyncio.Queue(), engine.model.forward
+
+    def planted(*a, **more):
+        out = forward(*a, **more)
+        out.logits[0, -1, 7] = float("nan")
+        return out
+
+    engine.model.forward = planted
+    got = together(engine, [("hello", 3, 0.0), ("there", 3, 0.5)])
+    assert isinstance(got[0], str) and isinstance(got[1], ValueError)
+    assert engine.paged.cache.free_count.tolist() == [engine.paged.cache.pages]

@@ -394,6 +394,42 @@ def test_prompt_attention_of_few_rows_over_many_keys(device, kind, cached, dim, 
 
 
 @both
+@pytest.mark.parametrize("requests", [64, 65, 130])
+@pytest.mark.parametrize("kind,cached,dim", [("bf16", "bf16", 128), ("fp16", "fp16", 64), ("bf16", "e4m3", 80)])
+def test_prompts_of_many_requests(device, kind, cached, dim, requests):
+    """As many as a server may admit at once, their keys not split: up to 64 are ordered by their lengths, more are not."""
+    rng = random.Random(requests)
+    gen = torch.Generator().manual_seed(requests + dim)
+    new = [rng.choice([0, 1, rng.randint(2, 90)]) for _ in range(requests)]
+    held = [rng.choice([0, 0, rng.randint(1, 120)]) for _ in range(requests)]
+    lens = [h + n for h, n in zip(held, new)]
+    cu = [0]
+    for n in new:
+        cu.append(cu[-1] + n)
+    cache = make_cache(gen, lens, 2, dim, 16, kind, cached, device)
+    q = torch.randn((cu[-1], 4, dim), generator=gen).to(TYPES[kind]).to(device)
+    check_attention(run_prompt(q, cache, lens, cu), q, cache, lens, cu)
+
+
+@both
+@pytest.mark.parametrize("kind,cached,dim", [("bf16", "bf16", 128), ("fp16", "fp16", 64), ("bf16", "e4m3", 80), ("bf16", "bf16", 256)])
+@pytest.mark.parametrize("lens", [[333], [1], [256, 0, 1, 17, 63], [300] * 32])
+def test_short_rows_of_a_table_as_wide_as_a_server_makes_it(device, kind, cached, dim, lens):
+    """Room for 2048 tokens a row: the operators choose their form by it. One token of each row, and the rows' whole prompts."""
+    gen = torch.Generator().manual_seed(len(lens) + dim)
+    k_cache, v_cache, tables, scales = make_cache(gen, lens, 2, dim, 64, kind, cached, device)
+    cache = (k_cache, v_cache, [t + [-1] * (32 - len(t)) for t in tables], scales)
+    q = torch.randn((sum(lens), 4, dim), generator=gen).to(TYPES[kind]).to(device)
+    one = torch.randn((len(lens), 4, dim), generator=gen).to(TYPES[kind]).to(device)
+    check_attention(run_decode(one, cache, lens), one, cache, lens, list(range(len(lens) + 1)))
+    if len(lens) < 32:
+        cu = [0]
+        for n in lens:
+            cu.append(cu[-1] + n)
+        check_attention(run_prompt(q, cache, lens, cu), q, cache, lens, cu)
+
+
+@both
 @pytest.mark.parametrize("dim", [64, 128])
 def test_split_keys_with_bad_entries_and_values(device, dim):
     """The same with an entry that names no page, and a later token that is not finite, in different parts of the keys."""
