@@ -287,7 +287,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : 4) void split_kernel(Sp
     }
   };
 
-  // One tile of registers, the table's entries a tile ahead: 126 registers, so that four waves share a SIMD and one
+  // One tile of registers, the table's entries a tile ahead: 125 registers, so that four waves share a SIMD and one
   // computes while the others' loads are on their way. A second tile (221 registers, two waves) measured 33.4 us
   // instead of 31.6 on 32 ragged rows up to 2048, 98.9 instead of 98.5 on one of 131071 (bf16, 8 kv heads of 128).
   constexpr int kStride = kWaves * kTile;
@@ -406,7 +406,7 @@ __global__ __launch_bounds__(kWaves * 64) void join_kernel(SplitArgs s) {
 // Keys of a chunk at least: shorter ones spend their time on starting and joining.
 constexpr int kLeast = 256;
 // Where no row can hold more keys, each is one chunk and nothing is joined: one launch instead of two. On one row of 333
-// keys 6.2 us, against 5.6 + 4.2 split in two.
+// keys 5.9 us, against 5.6 + 3.8 split in two.
 constexpr int kOne = 512;
 // Rows of the join (requests by heads) up to which a workgroup joins one head only, with many threads along the chunks.
 constexpr int kFewRows = 512;

@@ -385,7 +385,9 @@ __global__ __launch_bounds__(kWaves * 64, waves_of(D, sizeof(typename C::T) == 1
       for (int r = 0; r < 16; r++) {
         float y = __builtin_amdgcn_exp2f(__builtin_fmaf(x[h][r], a.score_scale, -from));
         l += y;
-        p[2 * h + (r >> 3)][r & 7] = (typename X::T)y;  // rounded for the matrix product; the sum l is not
+        // Rounded for the matrix product; the sum l is not. The error against 64 bits is 1.25 to 1.4 times that of rounding the
+        // result; what is left as a second part, as for one token, would be half as many products again.
+        p[2 * h + (r >> 3)][r & 7] = (typename X::T)y;
       }
   };
   auto v_operand = [&](int buffer, int step, int d) {
