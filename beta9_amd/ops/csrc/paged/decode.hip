@@ -307,7 +307,10 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 2 : 4) void split_kernel(Sp
   if (__any(m == kMinusInf)) {
     for (base = first + wave * kTile; base < last; base += kStride) {
       bool known = (unsigned)entry_of(base + v_key) < (unsigned)a.pages;
-      if (__any(known && base + v_key < last)) m = fmaxf(m, kLowest);
+      if (__any(known && base + v_key < last)) {
+        m = fmaxf(m, kLowest);
+        break;
+      }
     }
   }
   // the four waves' sums
